@@ -158,6 +158,60 @@ int zepp_lane_arm(const int64_t* swap_out_dev, int R, int rank, int nlp, int cap
  * limit_ms passed; result_dev[0] = 1 reached, 0 gave up.  Used to test the timeout path without a hang. */
 int zepp_wait_geq(const uint64_t* flag_dev, uint64_t value, int limit_ms, int32_t* result_dev, void* stream);
 
+/* ---- operators around the layer -----------------------------------------------------------------
+ * No counterpart in the reference, whose callers bring ids, weights and trained experts: the gate, tokens sorted by
+ * expert and back, the experts' products and the gradient norm, with their gradients.  Element types: 0 float32,
+ * 1 bfloat16, 2 float16.  Tensors are contiguous, row-major, on the current device and aligned to their elements.
+ * Outputs are written whole; workspaces belong to one call until its work on `stream` is done. */
+
+/* logits [T, G] -> ids [T, k] (largest first, equal ones by index; -1 where fewer than k experts can be chosen: a logit of
+ * -inf or NaN cannot) and weights [T, k].  sigmoid 0: softmax over the experts, 1: sigmoid scores.  renormalize: weights
+ * of a token sum to `scale`.  bias [G] (or null; sigmoid only) is added to the scores for the choice alone.
+ * G <= 1024, k <= min(32, G). */
+int zepp_op_gate(const void* logits_dev, int dtype, int64_t T, int G, int k, int sigmoid, int renormalize,
+                 const float* bias_dev, float scale, int32_t* ids_dev, float* weights_dev, void* stream);
+int zepp_op_gate_grad(const void* logits_dev, int dtype, int64_t T, int G, int k, int sigmoid, int renormalize,
+                      float scale, const int32_t* ids_dev, const float* weights_dev, const float* dweights_dev,
+                      void* dlogits_dev, void* stream);
+
+/* x [T, H] and ids [T, K] -> rows [T*K, H] in the order of (group, token, k), offsets [G + 1] (first row of each group; the
+ * last one: rows that hold a copy, those behind it are zero) and position [T, K] (a copy's row, -1 for a copy without a
+ * group).  The group of an id is group_of[id] (ids 0 .. n_ids - 1), or the id itself where group_of is null; ids and groups
+ * out of range have none.  ws: zepp_op_sort_ws_ints() int32.  K <= 64, G <= 2048, T*K < 2^31. */
+size_t zepp_op_sort_ws_ints(int64_t T, int K, int G);
+int zepp_op_sort(const void* x_dev, int dtype, int64_t T, int K, int64_t H, const int32_t* ids_dev,
+                 const int32_t* group_of_dev, int n_ids, int G, int32_t* ws_dev, void* rows_dev, int32_t* offsets_dev,
+                 int32_t* position_dev, void* stream);
+/* y [T, H]: sum over k of weights[t, k] * rows[position[t, k]], in fp32; weights null: 1 (the gradient of x in zepp_op_sort) */
+int zepp_op_unsort(const void* rows_dev, int dtype, int64_t T, int K, int64_t H, const int32_t* position_dev,
+                   const float* weights_dev, void* y_dev, void* stream);
+/* gradients of zepp_op_unsort: drows [T*K, H] (zero behind offsets[G]) and dweights [T, K]; either may be null */
+int zepp_op_unsort_grad(const void* dy_dev, const void* rows_dev, int dtype, int64_t T, int K, int64_t H, int G,
+                        const int32_t* offsets_dev, const int32_t* position_dev, const float* weights_dev, void* drows_dev,
+                        float* dweights_dev, void* stream);
+
+/* y [n, H] of rows [n, H] through expert e's w1 [G, f1, H], activation and w2 [G, H, I] for rows offsets[e] ..
+ * offsets[e + 1] (offsets[0] counts as 0; y is zero behind the last expert's rows).  bf16; act as in zepp_layer_cfg;
+ * f1 = 2 I (gate rows, then up rows) for swiglu, I for gelu; H and I multiples of 8, G <= 1024, tensors on 16-byte
+ * boundaries.  a [n, I] takes the activations; h [n, f1] the products before them, or null: no gradient wanted. */
+int zepp_op_expert_ffn(const void* rows_dev, int64_t n, const int32_t* offsets_dev, int G, int H, int I, int act,
+                       const void* w1_dev, const void* w2_dev, void* a_dev, void* h_dev, void* y_dev, void* stream);
+/* gradients from dy [n, H] and the forward call's a and h; dh_ws [n, f1] is a workspace; drows, dw1, dw2 may be null */
+int zepp_op_expert_ffn_grad(const void* dy_dev, const void* rows_dev, int64_t n, const int32_t* offsets_dev, int G, int H,
+                            int I, int act, const void* w1_dev, const void* w2_dev, const void* a_dev, const void* h_dev,
+                            void* dh_ws_dev, void* drows_dev, void* dw1_dev, void* dw2_dev, void* stream);
+
+/* norm [1] fp32: the 2-norm over all elements of `count` tensors (host arrays of device pointers, element counts and
+ * types).  max_norm >= 0: the tensors are then scaled in place by min(1, max_norm / (norm + 1e-6)); negative: they are
+ * only read.  The tensors must not overlap where they are scaled.  ws: zepp_op_grad_norm_ws_bytes(count). */
+size_t zepp_op_grad_norm_ws_bytes(int count);
+int zepp_op_grad_norm(void* const* ptrs, const int64_t* sizes, const uint8_t* dtypes, int count, double max_norm,
+                      float* norm_dev, void* ws_dev, void* stream);
+
+/* Deferred verdict of the operators' bounded waits on the current device: synchronises `stream`, copies 8 status words
+ * (as zepp_layer_status) and clears them. */
+int zepp_op_status(void* stream, uint64_t out[8]);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ loaded on first use and its absence is an error: there is no CPU path.
 """
 from . import config as _config
 from . import layer as _layer
+from . import ops as _ops
 
 SHAPES = _config.SHAPES
 ModelShape = _config.ModelShape
@@ -14,6 +15,14 @@ EPMoE = _layer.EPMoE
 Marks = _layer.Marks
 activation = _layer.activation
 token_buckets = _layer.token_buckets
+route_topk = _ops.route_topk
+sort_tokens = _ops.sort_tokens
+unsort_tokens = _ops.unsort_tokens
+SortPlan = _ops.SortPlan
+expert_ffn = _ops.expert_ffn
+grad_norm = _ops.grad_norm
+clip_grad_norm_ = _ops.clip_grad_norm_
 
-__all__ = ["SHAPES", "ModelShape", "EPMoEConfig", "tokens_per_rank", "EPMoE", "Marks", "activation", "token_buckets"]
+__all__ = ["SHAPES", "ModelShape", "EPMoEConfig", "tokens_per_rank", "EPMoE", "Marks", "activation", "token_buckets",
+           "route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_"]
 __version__ = "0.1.0"

@@ -4,7 +4,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "runtime.cu")
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("runtime.cu", "ops.cu")]
 OUT = os.path.join(HERE, "lib", "libzepp_b200.so")
 DEPS = [os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))] + \
        [os.path.join(os.path.dirname(HERE), "include", "zepp_b200.h")]
@@ -16,7 +16,7 @@ def build(force=False, verbose=False):
         return OUT
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--shared",
-           "-Xcompiler", "-fPIC", "-o", OUT, SRC]
+           "-t", str(len(SRCS)), "-Xcompiler", "-fPIC", "-o", OUT, *SRCS]
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]
     extra = os.environ.get("ZEPP_B200_NVCC_FLAGS", "").split()     # e.g. -DZEPP_FINE_TRACE, -DZEPP_GEMM_PROFILE

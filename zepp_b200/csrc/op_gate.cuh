@@ -1,0 +1,274 @@
+// The gate: top-k experts of each token and their weights from the router's logits, and the gradient of the weights.
+//
+//   softmax:  p = exp(l - max l) / sum exp(l - max l);   w_j = scale * p_{i_j},  renormalised: scale * p_{i_j} / sum_c p_{i_c}
+//   sigmoid:  s = 1 / (1 + exp(-l));                     w_j = scale * s_{i_j},  renormalised: scale * s_{i_j} / (sum_c s_{i_c} + 1e-20)
+//
+// i_1 .. i_k are the experts with the largest logits (softmax and sigmoid are monotone, so no rounding of theirs decides
+// between two experts), or with the largest s + bias where a balancing bias is given; equal values go to the lowest
+// index.  A logit of -inf or NaN is never chosen; a row with fewer than k others has id -1 and weight 0 in the last
+// places, and a NaN anywhere in a row makes its weights NaN.
+//
+// A warp owns a row and holds it in registers, so the logits are read once: element (j / 4) * 128 + lane * 4 + j % 4 for
+// register j, four neighbours per access.  Each of the k rounds takes the maximum of an order-preserving integer key with
+// redux.sync and the lowest index that has it with a second one; only the winner's lane looks through its registers
+// again.  Bound by instruction issue from about 8 rounds on, by the bytes of the logits below that.
+#pragma once
+#include "op_common.cuh"
+
+namespace zepp {
+
+constexpr int kGateWarps = 4;
+constexpr int kGateMaxExperts = 1024;
+constexpr int kGateMaxK = 32;            // lane j of the row's warp keeps the j-th choice
+
+struct GateArgs {
+  const void* logits;     // [T, G]
+  long long T;
+  int G, k;
+  int sigmoid, renormalize;
+  const float* bias;      // [G] or nullptr
+  float scale;
+  int* ids;               // [T, k]
+  float* weights;         // [T, k]
+  // gradient
+  const float* dweights;  // [T, k]
+  void* dlogits;          // [T, G]
+  int vec;                // rows can be accessed four elements at a time
+};
+
+__device__ __forceinline__ unsigned gate_key(float v) {      // larger key <=> larger value; 0: not to be chosen
+  v += 0.0f;                                                 // -0 and +0 are equal
+  const unsigned b = __float_as_uint(v);
+  return v > -INFINITY ? ((b >> 31) ? ~b : (b | 0x80000000u)) : 0u;
+}
+__device__ __forceinline__ float gate_value(unsigned key) {
+  return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
+}
+__device__ __forceinline__ int gate_index(int lane, int j) { return (j >> 2) * 128 + lane * 4 + (j & 3); }
+
+template <typename T, int NPL>
+__device__ __forceinline__ void gate_load(const T* row, int G, int lane, bool vec, float (&v)[NPL], float fill) {
+#pragma unroll
+  for (int q = 0; q < NPL / 4; ++q) {
+    const int i = gate_index(lane, 4 * q);
+    if (vec) {
+      if (i < G) {
+        const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(row + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = to_f32<T>(p.v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = fill;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < G ? to_f32<T>(row[i + e]) : fill;
+    }
+  }
+}
+
+__device__ __forceinline__ float sigmoid_f32(float l) { return 1.0f / (1.0f + expf(-l)); }
+
+// The choice by s + bias in 64 bits, for rows where two neighbours of the order lie within the rounding of the 32-bit
+// values: lane j < k returns its choice, -1 where none is left.
+template <int NPL>
+__device__ __noinline__ int gate_choose_f64(const float (&l)[NPL], const float* bias, int G, int k, int lane) {
+  double key[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const int i = gate_index(lane, j);
+    key[j] = -INFINITY;
+    if (i < G && l[j] > -INFINITY) {
+      const double v = 1.0 / (1.0 + exp(-(double)l[j])) + (double)bias[i];
+      if (v > -INFINITY) key[j] = v;                 // false for NaN
+    }
+  }
+  int mine = -1;
+  for (int r = 0; r < k; ++r) {
+    double best = -INFINITY;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const double ob = __shfl_xor_sync(0xffffffffu, best, o);
+      const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+      if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
+    }
+    if (!(best > -INFINITY)) break;
+    if (lane == r) mine = at;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (gate_index(lane, j) == at) key[j] = -INFINITY;
+  }
+  return mine;
+}
+
+template <typename T, int NPL>
+__global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a) {
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * kGateWarps + (threadIdx.x >> 5);
+  if (row >= a.T) return;
+  const T* src = static_cast<const T*>(a.logits) + row * a.G;
+  float l[NPL];
+  gate_load<T, NPL>(src, a.G, lane, a.vec, l, -INFINITY);
+  unsigned key[NPL];
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    nan |= l[j] != l[j];
+    float v = l[j];
+    if (a.bias != nullptr) {
+      const int i = gate_index(lane, j);
+      v = l[j] > -INFINITY ? sigmoid_f32(l[j]) + a.bias[i < a.G ? i : 0] : -INFINITY;
+    }
+    key[j] = gate_key(v);
+  }
+  nan = __any_sync(0xffffffffu, nan);
+
+  int mine = -1;                 // lane j < k: the j-th choice
+  unsigned top = 0, last = 0;    // the largest key of the row; the key of the round before
+  bool doubt = false;
+  unsigned best = 0;
+  int at = 0;                    // this lane's largest key and the lowest index that has it
+#pragma unroll
+  for (int j = 0; j < NPL; ++j)
+    if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
+  const int rounds = a.bias != nullptr ? a.k + 1 : a.k;      // one more shows how far behind the next expert is
+  for (int r = 0; r < rounds; ++r) {
+    const unsigned m = __reduce_max_sync(0xffffffffu, best);
+    if (m == 0u) break;
+    const int i = (int)__reduce_min_sync(0xffffffffu, best == m ? (unsigned)at : 0x7fffffffu);
+    if (r == 0) top = m;
+    if (a.bias != nullptr) {
+      // the 32-bit score is off by at most 2.5 units of 2^-24 for the exponential, one each for the sum, the quotient
+      // and the addition of the bias (relative to |s + b|): 4e-7 covers both sides of a comparison of s <= 1
+      const float v = gate_value(m);
+      if (r > 0 && gate_value(last) - v <= 8e-7f + 2.4e-7f * fabsf(v)) doubt = true;
+      last = m;
+    }
+    if (lane == r && r < a.k) mine = i;
+    if (at == i && best == m) {
+      best = 0;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        if (gate_index(lane, j) == i) key[j] = 0;
+        if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
+      }
+    }
+  }
+  if (doubt) mine = gate_choose_f64<NPL>(l, a.bias, a.G, a.k, lane);
+
+  const float lc = mine >= 0 ? to_f32<T>(src[mine]) : 0.0f;
+  float w = 0.0f;
+  if (a.sigmoid) {
+    w = mine >= 0 ? sigmoid_f32(lc) : 0.0f;
+    if (a.renormalize) w /= warp_sum(w) + 1e-20f;
+  } else {
+    const float mx = top ? gate_value(top) : 0.0f;           // NaN is left out of it: the row is marked below
+    w = mine >= 0 ? expf(lc - mx) : 0.0f;
+    float sum;
+    if (a.renormalize) {
+      sum = warp_sum(w);
+    } else {
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) sum += expf(l[j] - mx);
+      sum = warp_sum(sum);
+    }
+    if (mine >= 0) w /= sum;
+  }
+  w *= a.scale;
+  if (nan) w = __int_as_float(0x7fffffff);
+  if (lane < a.k) {
+    a.ids[row * a.k + lane] = mine;
+    a.weights[row * a.k + lane] = w;
+  }
+}
+
+// With q_c = scale * dw_c of the chosen experts c:
+//   softmax, all experts:   dl_g = p_g * (q_g [g chosen] - sum_c q_c p_c)
+//   renormalised, t = sum_c v_c, v = p or s:  dv_c = (q_c - sum_e q_e v_e / t) / t;  dl_c = dv_c v_c (softmax), dv_c s_c (1 - s_c)
+//   sigmoid, not renormalised:  dl_c = q_c s_c (1 - s_c)
+// Only the first has a value for every expert; the others write zeros there and read the chosen logits alone.
+template <typename T, int NPL>
+__global__ void __launch_bounds__(32 * kGateWarps) gate_grad_kernel(const GateArgs a) {
+  extern __shared__ __align__(16) unsigned char gate_rows[];       // kGateWarps rows of G elements, 16-byte multiples
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * kGateWarps + warp;
+  if (row >= a.T) return;
+  const T* src = static_cast<const T*>(a.logits) + row * a.G;
+  T* dst = static_cast<T*>(a.dlogits) + row * a.G;
+  int id = -1;
+  float q = 0.0f, w = 0.0f;
+  if (lane < a.k) {
+    id = a.ids[row * a.k + lane];
+    w = a.weights[row * a.k + lane];
+    if (id >= a.G) id = -1;
+    if (id >= 0) q = a.scale * a.dweights[row * a.k + lane];
+  }
+  const float lc = id >= 0 ? to_f32<T>(src[id]) : -INFINITY;
+  float mine;                                                     // dl of this lane's chosen expert
+  float p[NPL];
+  if (!a.sigmoid && !a.renormalize) {
+    gate_load<T, NPL>(src, a.G, lane, a.vec, p, -INFINITY);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) mx = fmaxf(mx, p[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (mx == -INFINITY) mx = 0.0f;                               // every expert masked: exp(-inf) = 0 below
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) { p[j] = expf(p[j] - mx); sum += p[j]; }
+    sum = warp_sum(sum);
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const float pc = id >= 0 ? expf(lc - mx) * inv : 0.0f;
+    const float dot = warp_sum(q * pc);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) p[j] *= -inv * dot;
+    mine = pc * (q - dot);
+  } else {
+    float v, slope;
+    if (a.sigmoid) {
+      v = id >= 0 ? sigmoid_f32(lc) : 0.0f;
+      slope = id >= 0 ? v * sigmoid_f32(-lc) : 0.0f;
+    } else {
+      float mx = lc;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      v = id >= 0 ? expf(lc - mx) : 0.0f;
+      slope = v;
+    }
+    float d = q;
+    if (a.renormalize) {
+      const float t = warp_sum(v) + (a.sigmoid ? 1e-20f : 0.0f);
+      const float dot = warp_sum(q * v);
+      if (t > 0.0f) d = (q - dot / t) / t;
+    }
+    mine = id >= 0 ? d * slope : 0.0f;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) p[j] = 0.0f;
+  }
+  if (w != w) mine = w;                                           // a row that held NaN
+  // the row is put together in shared memory, so that it leaves in whole vectors with the chosen values in their places
+  T* st = reinterpret_cast<T*>(gate_rows) + (size_t)warp * ((a.G + 7) / 8 * 8);
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const int i = gate_index(lane, j);
+    if (i < a.G) st[i] = from_f32<T>(p[j]);
+  }
+  __syncwarp();
+  if (id >= 0) st[id] = from_f32<T>(mine);
+  __syncwarp();
+  if (a.vec) {
+    for (int i = lane * 4; i < a.G; i += 128)
+      *reinterpret_cast<Pack<T, 4>*>(dst + i) = *reinterpret_cast<const Pack<T, 4>*>(st + i);
+  } else {
+    for (int i = lane; i < a.G; i += 32) dst[i] = st[i];
+  }
+}
+
+}  // namespace zepp

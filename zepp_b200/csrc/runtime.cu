@@ -17,6 +17,7 @@
 #include "front.cuh"
 #include "gemm.cuh"
 #include "gemm_pair.cuh"
+#include "host.cuh"
 #include "layer_kernels.cuh"
 #include "meta.cuh"
 #include "planner.cuh"
@@ -31,7 +32,7 @@ constexpr int kSwapCap = 8;        // expert moves per rank and step (the refere
 // ---------------------------------------------------------------------------------------------
 static thread_local std::string g_err;
 
-static int fail(const char* fmt, ...) {
+int zepp::fail(const char* fmt, ...) {
   char buf[1024];
   va_list ap;
   va_start(ap, fmt);
@@ -40,12 +41,6 @@ static int fail(const char* fmt, ...) {
   g_err = buf;
   return 1;
 }
-
-#define CU_OK(expr)                                                                         \
-  do {                                                                                      \
-    cudaError_t _e = (expr);                                                                \
-    if (_e != cudaSuccess) return fail("%s failed: %s (%s:%d)", #expr, cudaGetErrorString(_e), __FILE__, __LINE__); \
-  } while (0)
 
 static int swap_decide_prepare();
 static SwapArgs swap_args(const int* loads, int* p2l, int* l2p, const int* lcnts, int R, int G, int L, int nlp, double C,
@@ -173,11 +168,7 @@ extern "C" int zepp_rt_sm_count(zepp_rt* rt) { return rt->sm_count; }
 // ---------------------------------------------------------------------------------------------
 // tensor maps
 // ---------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn zepp::encode_fn() {
   static EncodeTiledFn fn = nullptr;
   if (fn) return fn;
   void* p = nullptr;

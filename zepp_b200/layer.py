@@ -14,7 +14,7 @@ device planning needs two or more nodes (python/zepp/layer.py:66), device planni
 """
 import torch
 
-from . import constants
+from . import constants, ops
 from .capacity import CapacityExceeded, Demands, violations
 from .config import EPMoEConfig
 from .placement import Placement, demand_histogram, solve_placement
@@ -120,6 +120,7 @@ class EPMoE(torch.nn.Module):
         self._plan_views = None
         self._tokens = cfg.max_tokens_per_rank        # the bucket the next step runs at
         self._pad_bufs = {}
+        self._group_of = None                         # local group of each expert (forward_train)
 
     @staticmethod
     def arena_bytes(cfg, caps):
@@ -268,6 +269,40 @@ class EPMoE(torch.nn.Module):
         self._h.step(ids, wts, x.contiguous(), y)
         self._epoch += 1
         return y
+
+    # -- gate and training ------------------------------------------------------------------
+    def gate(self, logits, score="softmax", renormalize=True, bias=None, scale=1.0):
+        """The router's logits [tokens, E] -> (ids, weights) as prepare() and step() take them: see ops.route_topk.
+        A row masked out with -inf is a pad row (ids -1)."""
+        assert logits.dim() == 2 and logits.shape[1] == self.cfg.shape.num_experts, tuple(logits.shape)
+        return ops.route_topk(logits, self.cfg.shape.topk, score=score, renormalize=renormalize, bias=bias, scale=scale)
+
+    def train_weights(self):
+        """The expert weights as leaves that take gradients: [w1 [groups, ffn1, H], w2 [groups, H, ffn]], the tensors that
+        step() reads, so an optimizer that updates them in place serves both.  Unused slots get zero gradients."""
+        assert self.w1 is not None, "load_weights / set_weights first"
+        return [self.w1.requires_grad_(True), self.w2.requires_grad_(True)]
+
+    def forward_train(self, x, topk_ids, topk_weights):
+        """y of the layer for any number of tokens x [n, H], differentiable in x, topk_weights and (after train_weights())
+        the expert weights: sort by expert -> the experts' products -> back with the weights applied.  Layers of one rank,
+        without swap.  Agrees with step() to bf16 rounding: the activations and the weighted sum keep fp32 where step()
+        rounds as the reference does."""
+        cfg, shape = self.cfg, self.cfg.shape
+        assert cfg.ranks == 1 and not cfg.swap, "forward_train: layers of one rank, without swap"
+        assert self.w1 is not None, "load_weights / set_weights first"
+        assert x.shape == (topk_ids.shape[0], shape.hidden) and topk_ids.shape[1] == shape.topk, (tuple(x.shape), tuple(topk_ids.shape))
+        if self._group_of is None:       # group 0 is the pad group; on one rank every expert has one slot
+            self._group_of = (1 + self.placement.l2p[:, 0]).to(device=self.device, dtype=torch.int32)
+        rows, plan = ops.sort_tokens(x, topk_ids.to(torch.int32), cfg.groups_per_rank, group_of=self._group_of)
+        rows = ops.expert_ffn(rows, plan.offsets, self.w1, self.w2, act=shape.act)
+        return ops.unsort_tokens(rows, plan, topk_weights.float())
+
+    def clip_grad_norm_(self, max_norm, others=()):
+        """Scale the gradients of the expert weights and of `others` (parameters, such as the router's) in place to at
+        most max_norm together; returns their norm.  Parameters without a gradient are left out."""
+        params = [p for p in (self.w1, self.w2, *others) if p is not None]
+        return ops.clip_grad_norm_([p.grad for p in params if p.grad is not None], max_norm)
 
     # -- verdict ----------------------------------------------------------------------------
     def check(self):

@@ -1,0 +1,391 @@
+"""Operators around the expert-parallel layer, with gradients: what makes its ids and weights, and what trains its experts.
+
+    ids, weights = route_topk(logits, k)                  # the gate
+    rows, plan = sort_tokens(x, ids, num_experts)         # a row for every copy, by expert
+    rows = expert_ffn(rows, plan.offsets, w1, w2)         # the experts' products and activation
+    y = unsort_tokens(rows, plan, weights)                # back, with the weights applied
+    norm = clip_grad_norm_(gradients, max_norm)           # the norm of all gradients, and clipping
+
+Each call is one to five kernels of libzepp_b200.so on the current stream of its tensors' device; nothing is read back
+on the host, and calls can be captured into CUDA graphs after one call on that device outside of a capture.  Arguments
+that do not fit are refused with an AssertionError, as everywhere in this package.  Inputs that are not contiguous (or,
+for expert_ffn, not on a 16-byte boundary) are copied.  Gradients are first derivatives only.
+
+Where a backward pass is captured into a graph, make the forward pass that it belongs to inside the same capture, of
+leaves that no graph outside of it still holds (torch runs a leaf's accumulation on the stream of the leaf's first use).
+"""
+import ctypes
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ._ext import check, lib
+
+__all__ = ["route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_", "check_waits"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_ACTS = {"gelu": 0, "swiglu": 1}
+MAX_GATE_EXPERTS, MAX_GATE_TOPK = 1024, 32
+MAX_SORT_EXPERTS, MAX_SORT_TOPK = 2048, 64
+MAX_FFN_EXPERTS = 1024
+
+_P, _I, _L, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
+_ARGS = {
+    "zepp_op_gate": (_P, _I, _L, _I, _I, _I, _I, _P, _F, _P, _P, _P),
+    "zepp_op_gate_grad": (_P, _I, _L, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P),
+    "zepp_op_sort_ws_ints": (_L, _I, _I),
+    "zepp_op_sort": (_P, _I, _L, _I, _L, _P, _P, _I, _I, _P, _P, _P, _P, _P),
+    "zepp_op_unsort": (_P, _I, _L, _I, _L, _P, _P, _P, _P),
+    "zepp_op_unsort_grad": (_P, _P, _I, _L, _I, _L, _I, _P, _P, _P, _P, _P, _P),
+    "zepp_op_expert_ffn": (_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P),
+    "zepp_op_expert_ffn_grad": (_P, _P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P),
+    "zepp_op_grad_norm_ws_bytes": (_I,),
+    "zepp_op_grad_norm": (_P, _P, _P, _I, _D, _P, _P, _P),
+    "zepp_op_status": (_P, _P),
+}
+_SIZES = ("zepp_op_sort_ws_ints", "zepp_op_grad_norm_ws_bytes")
+_fns = {}
+
+
+def _fn(name):
+    f = _fns.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes = _ARGS[name]
+        f.restype = ctypes.c_size_t if name in _SIZES else ctypes.c_int
+        _fns[name] = f
+    return f
+
+
+def _refuse(what):
+    raise AssertionError(what)
+
+
+def _call(name, device, *args):
+    """One entry point on the current stream of `device`."""
+    if device.index == torch.cuda.current_device():
+        rc = _fn(name)(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = _fn(name)(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        check(rc)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            _refuse(f"{name} is on {t.device}, not on {device}")
+
+
+# ------------------------------------------------------------------------------------------------ gate
+def _gate(logits, k, score, renormalize, bias, scale):
+    T, G = logits.shape
+    ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+    _call("zepp_op_gate", logits.device, logits.data_ptr(), _TYPES[logits.dtype], T, G, k, score, renormalize, _ptr(bias),
+          scale, ids.data_ptr(), weights.data_ptr())
+    return ids, weights
+
+
+class _Gate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, score, renormalize, bias, scale):
+        ids, weights = _gate(logits, k, score, renormalize, bias, scale)
+        ctx.save_for_backward(logits, ids, weights)
+        ctx.how = (k, score, renormalize, scale)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return ids, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, dweights):
+        if dweights is None:
+            return (None,) * 6
+        logits, ids, weights = ctx.saved_tensors
+        k, score, renormalize, scale = ctx.how
+        dlogits = torch.empty_like(logits)
+        dweights = dweights.contiguous()
+        _call("zepp_op_gate_grad", logits.device, logits.data_ptr(), _TYPES[logits.dtype], logits.shape[0], logits.shape[1], k,
+              score, renormalize, scale, ids.data_ptr(), weights.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
+        return dlogits, None, None, None, None, None
+
+
+def route_topk(logits, k, score="softmax", renormalize=True, bias=None, scale=1.0):
+    """The gate: ids [T, k] int32 of the k experts with the largest logits (largest first, equal ones by index) and their
+    weights [T, k] float32, differentiable in the logits [T, E] (float32, bfloat16 or float16).
+
+    score="softmax": a weight is the expert's probability over all experts; "sigmoid": the sigmoid of its logit.
+    renormalize divides a token's weights by their sum; scale multiplies them.  bias [E] float32 (sigmoid only) is added
+    to the scores for the choice alone and gets no gradient.  Experts whose logit is -inf or NaN are not chosen: a token
+    that has fewer than k others gets id -1 and weight 0 in its last places (a token masked out altogether is a pad row of
+    the layer).  A NaN in a row makes its weights NaN.  E <= 1024, k <= min(32, E)."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _TYPES:
+        _refuse(f"logits: a CUDA tensor [tokens, experts] of float32, bfloat16 or float16, got {tuple(logits.shape)} {logits.dtype} {logits.device}")
+    G = logits.shape[1]
+    if not 1 <= G <= MAX_GATE_EXPERTS or not 1 <= k <= min(MAX_GATE_TOPK, G):
+        _refuse(f"1..{MAX_GATE_EXPERTS} experts and top-k of 1..min({MAX_GATE_TOPK}, experts), got {G} and {k}")
+    if score not in _SCORES:
+        _refuse(f"score: one of {tuple(_SCORES)}, got {score!r}")
+    if bias is not None:
+        if score != "sigmoid" or bias.shape != (G,) or bias.dtype != torch.float32:
+            _refuse("bias: float32 [experts], with sigmoid scores")
+        _on(logits.device, bias=bias)
+        bias = bias.detach().contiguous()
+    logits = logits.contiguous()
+    args = (logits, int(k), _SCORES[score], int(bool(renormalize)), bias, float(scale))
+    return _Gate.apply(*args) if logits.requires_grad and torch.is_grad_enabled() else _gate(*args)
+
+
+# ----------------------------------------------------------------------------------- sort by expert and back
+class SortPlan(NamedTuple):
+    """Where the copies of sort_tokens' tokens are: rows offsets[e] .. offsets[e + 1] belong to expert e (int32
+    [experts + 1], the last one is the number of rows that hold a copy), position [T, K] int32 is a copy's row or -1."""
+    offsets: torch.Tensor
+    position: torch.Tensor
+
+
+def _sort(x, ids, num_experts, group_of):
+    T, K = ids.shape
+    H = x.shape[1]
+    rows = torch.empty((T * K, H), dtype=x.dtype, device=x.device)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=x.device)
+    position = torch.empty((T, K), dtype=torch.int32, device=x.device)
+    ints = _fn("zepp_op_sort_ws_ints")(T, K, num_experts)
+    ws = torch.empty(ints, dtype=torch.int32, device=x.device) if ints else None
+    _call("zepp_op_sort", x.device, x.data_ptr(), _TYPES[x.dtype], T, K, H, ids.data_ptr(), _ptr(group_of),
+          0 if group_of is None else group_of.shape[0], num_experts, _ptr(ws), rows.data_ptr(), offsets.data_ptr(),
+          position.data_ptr())
+    return rows, offsets, position
+
+
+def _unsort(rows, position, weights):
+    T, K = position.shape
+    H = rows.shape[1]
+    y = torch.empty((T, H), dtype=rows.dtype, device=rows.device)
+    _call("zepp_op_unsort", rows.device, rows.data_ptr(), _TYPES[rows.dtype], T, K, H, position.data_ptr(), _ptr(weights), y.data_ptr())
+    return y
+
+
+class _Sort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ids, num_experts, group_of):
+        rows, offsets, position = _sort(x, ids, num_experts, group_of)
+        ctx.save_for_backward(position)
+        ctx.mark_non_differentiable(offsets, position)
+        ctx.set_materialize_grads(False)
+        return rows, offsets, position
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows, _offsets, _position):
+        if drows is None:
+            return None, None, None, None
+        position, = ctx.saved_tensors
+        return _unsort(drows.contiguous(), position, None), None, None, None
+
+
+class _Unsort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, offsets, position, weights):
+        ctx.save_for_backward(rows if weights is not None and ctx.needs_input_grad[3] else None, offsets, position, weights)
+        ctx.like = (rows.shape, rows.dtype)
+        return _unsort(rows, position, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, offsets, position, weights = ctx.saved_tensors
+        dy = dy.contiguous()
+        T, K = position.shape
+        shape, dtype = ctx.like
+        drows = torch.empty(shape, dtype=dtype, device=dy.device) if ctx.needs_input_grad[0] else None
+        dweights = torch.empty((T, K), dtype=torch.float32, device=dy.device) if ctx.needs_input_grad[3] else None
+        _call("zepp_op_unsort_grad", dy.device, dy.data_ptr(), _ptr(rows), _TYPES[dtype], T, K, shape[1], offsets.shape[0] - 1,
+              offsets.data_ptr(), position.data_ptr(), _ptr(weights), _ptr(drows), _ptr(dweights))
+        return drows, None, None, dweights
+
+
+def sort_tokens(x, ids, num_experts, group_of=None):
+    """Rows of x [T, H] (float32, bfloat16 or float16), one for every copy, sorted by expert: (rows [T*K, H], SortPlan).
+    Copies of an expert keep the order of (token, k).  ids [T, K] int32; a copy whose id is not one of the experts
+    (the layer's pads have -1) gets no row, and rows that no copy fills are zero, at the end.  group_of: an int32 table
+    that names the group of each id (such as a layer's slot of each expert); `num_experts` then counts groups.
+    Differentiable in x.  K <= 64, at most 2048 experts, T*K < 2^31."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in _TYPES or x.shape[1] < 1:
+        _refuse(f"x: a CUDA tensor [tokens, hidden] of float32, bfloat16 or float16, got {tuple(x.shape)} {x.dtype} {x.device}")
+    if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[0] != x.shape[0] or not 1 <= ids.shape[1] <= MAX_SORT_TOPK:
+        _refuse(f"ids: int32 [{x.shape[0]}, 1..{MAX_SORT_TOPK}], got {tuple(ids.shape)} {ids.dtype}")
+    if not 1 <= num_experts <= MAX_SORT_EXPERTS:
+        _refuse(f"1..{MAX_SORT_EXPERTS} experts, got {num_experts}")
+    if group_of is not None:
+        if group_of.dim() != 1 or group_of.dtype != torch.int32:
+            _refuse("group_of: a table of int32")
+        group_of = group_of.contiguous()
+    _on(x.device, ids=ids, group_of=group_of)
+    args = (x.contiguous(), ids.contiguous(), int(num_experts), group_of)
+    rows, offsets, position = _Sort.apply(*args) if x.requires_grad and torch.is_grad_enabled() else _sort(*args)
+    return rows, SortPlan(offsets, position)
+
+
+def unsort_tokens(rows, plan, weights=None):
+    """The inverse of sort_tokens: y [T, H], y[t] = sum over k of weights[t, k] * rows[plan.position[t, k]] over the copies
+    that have a row, added up in float32 in the order of k.  weights [T, K] float32; without them every copy counts once.
+    Differentiable in rows and weights."""
+    T, K = plan.position.shape
+    if rows.dim() != 2 or not rows.is_cuda or rows.dtype not in _TYPES or rows.shape[0] != T * K or rows.shape[1] < 1:
+        _refuse(f"rows: [{T * K}, hidden] of float32, bfloat16 or float16, got {tuple(rows.shape)} {rows.dtype} {rows.device}")
+    if plan.position.dtype != torch.int32 or plan.offsets.dtype != torch.int32 or not 1 <= K <= MAX_SORT_TOPK:
+        _refuse("plan: as sort_tokens returns it")
+    if weights is not None:
+        if weights.shape != (T, K) or weights.dtype != torch.float32:
+            _refuse(f"weights: float32 [{T}, {K}], got {tuple(weights.shape)} {weights.dtype}")
+        weights = weights.contiguous()
+    _on(rows.device, position=plan.position, offsets=plan.offsets, weights=weights)
+    rows = rows.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Unsort.apply(rows, plan.offsets.contiguous(), plan.position.contiguous(), weights)
+    return _unsort(rows, plan.position.contiguous(), weights)
+
+
+# -------------------------------------------------------------------------------------------- experts' products
+def _dense16(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ffn(rows, offsets, w1, w2, act, keep):
+    n, H = rows.shape
+    G, f1 = w1.shape[:2]
+    I = w2.shape[2]
+    new = lambda c: torch.empty((n, c), dtype=torch.bfloat16, device=rows.device)  # noqa: E731
+    y, a, h = new(H), new(I), new(f1) if keep else None
+    _call("zepp_op_expert_ffn", rows.device, rows.data_ptr(), n, offsets.data_ptr(), G, H, I, act, w1.data_ptr(), w2.data_ptr(),
+          a.data_ptr(), _ptr(h), y.data_ptr())
+    return y, a, h
+
+
+class _ExpertFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, offsets, w1, w2, act):
+        y, a, h = _ffn(rows, offsets, w1, w2, act, True)
+        ctx.save_for_backward(rows, offsets, w1, w2, a, h)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, offsets, w1, w2, a, h = ctx.saved_tensors
+        n, H = rows.shape
+        G, f1 = w1.shape[:2]
+        need = ctx.needs_input_grad
+        dy = _dense16(dy)
+        drows = torch.empty_like(rows) if need[0] else None
+        dw1 = torch.empty_like(w1) if need[2] else None
+        dw2 = torch.empty_like(w2) if need[3] else None
+        dh = torch.empty((n, f1), dtype=torch.bfloat16, device=rows.device) if need[0] or need[2] else None
+        _call("zepp_op_expert_ffn_grad", rows.device, dy.data_ptr(), rows.data_ptr(), n, offsets.data_ptr(), G, H, w2.shape[2],
+              ctx.act, w1.data_ptr(), w2.data_ptr(), a.data_ptr(), h.data_ptr(), _ptr(dh), _ptr(drows), _ptr(dw1), _ptr(dw2))
+        return drows, None, dw1, dw2, None
+
+
+def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
+    """Each expert's two products and the activation between them on its own rows: y [n, H] of rows [n, H], where rows
+    offsets[e] .. offsets[e + 1] go through w1[e] [ffn1, H] and w2[e] [H, ffn] (ffn1 = 2 ffn for "swiglu": gate rows, then
+    up rows, as the layer holds them; ffn for "gelu").  All bfloat16, accumulated in float32; offsets int32 [experts + 1]
+    on the device, not decreasing, starting at 0; rows behind the last expert's give zero.  hidden and ffn are
+    multiples of 8; at most 1024 experts.  Differentiable in rows, w1 and w2; an expert without rows has a zero gradient."""
+    if act not in _ACTS:
+        _refuse(f"act: one of {tuple(_ACTS)}, got {act!r}")
+    if not rows.is_cuda or rows.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
+        _refuse(f"rows [n, hidden], w1 [experts, ffn1, hidden], w2 [experts, hidden, ffn] on a GPU, got {tuple(rows.shape)}, "
+                f"{tuple(w1.shape)}, {tuple(w2.shape)} on {rows.device}")
+    G, H, I = w2.shape
+    if rows.shape[1] != H or w1.shape != (G, I * (2 if act == "swiglu" else 1), H) or offsets.shape != (G + 1,):
+        _refuse(f"shapes do not fit: rows {tuple(rows.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}, offsets {tuple(offsets.shape)}, {act}")
+    if rows.dtype != torch.bfloat16 or w1.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16 or offsets.dtype != torch.int32:
+        _refuse("rows and weights are bfloat16, offsets int32")
+    if H % 8 or I % 8 or H < 8 or I < 8 or not 1 <= G <= MAX_FFN_EXPERTS:
+        _refuse(f"hidden and ffn are multiples of 8, 1..{MAX_FFN_EXPERTS} experts, got {H}, {I}, {G}")
+    _on(rows.device, offsets=offsets, w1=w1, w2=w2)
+    args = (_dense16(rows), offsets.contiguous(), _dense16(w1), _dense16(w2), _ACTS[act])
+    if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
+        return _ExpertFFN.apply(*args)
+    return _ffn(*args, False)[0]
+
+
+# ---------------------------------------------------------------------------------- norm of all gradients, clipping
+def _is_dense(t):
+    """Every element of the tensor's span belongs to it once, whatever the order of its dimensions."""
+    need = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+def _norm(tensors, max_norm):
+    tensors = list(tensors)
+    if not tensors:
+        _refuse("no tensors")
+    device = tensors[0].device
+    types = [_TYPES.get(t.dtype, -1) for t in tensors]
+    if device.type != "cuda" or min(types) < 0 or any(t.device != device for t in tensors):
+        _refuse("CUDA tensors of one device, of float32, bfloat16 or float16")
+    ptrs = [t.data_ptr() for t in tensors]
+    sizes = [t.numel() for t in tensors]
+    if not all(t.is_contiguous() or _is_dense(t) for t in tensors if t.numel()):
+        _refuse("tensors whose elements lie without gaps and only once in memory")
+    if max_norm >= 0:
+        last = 0
+        for p, n, ty in sorted(zip(ptrs, sizes, types)):
+            if n:
+                if p < last:
+                    _refuse("tensors that do not overlap (one is given twice?)")
+                last = p + n * (2 if ty else 4)
+    n = len(tensors)
+    out = torch.empty((), dtype=torch.float32, device=device)
+    ws = torch.empty(_fn("zepp_op_grad_norm_ws_bytes")(n), dtype=torch.uint8, device=device)
+    _call("zepp_op_grad_norm", device, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*sizes), bytes(types), n,
+          max_norm, out.data_ptr(), ws.data_ptr())
+    return out
+
+
+@torch.no_grad()
+def grad_norm(tensors):
+    """The 2-norm over all elements of the tensors (float32, bfloat16 and float16 may be mixed), a float32 scalar on their
+    device; sums run in 64 bits across chunks and in a fixed order."""
+    return _norm(tensors, -1.0)
+
+
+@torch.no_grad()
+def clip_grad_norm_(tensors, max_norm):
+    """Scale the tensors in place by min(1, max_norm / (norm + 1e-6)), norm being grad_norm(tensors), which is returned.
+    With a norm of NaN every element becomes NaN; with an infinite one the finite elements become 0.  The tensors must not
+    overlap; other orders of their dimensions are fine, gaps are not."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        _refuse(f"max_norm: not negative, got {max_norm}")
+    tensors = list(tensors)
+    out = _norm(tensors, max_norm)
+    torch.autograd.graph.increment_version(tensors)      # graphs that saved a tensor learn that it changed
+    return out
+
+
+def check_waits(device=None):
+    """Synchronise and raise if a bounded wait of an operator's kernel on `device` (default: the current one) ran out."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    out = (ctypes.c_uint64 * 8)()
+    with torch.cuda.device(device):
+        check(_fn("zepp_op_status")(torch.cuda.current_stream().cuda_stream, ctypes.addressof(out)))
+    if out[0]:
+        raise RuntimeError(f"zepp_b200 operator failed: a device-side wait ran out (wait id {out[1]}, item {out[2]}, step {out[3]})")
