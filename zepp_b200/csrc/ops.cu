@@ -305,10 +305,10 @@ static int ffn_rows_launch(const FfnCall& c, const void* rows, int K, const void
   a.feat = MODE == FFN_UP_SWIGLU ? 128 : 256;
   a.up_offset = MODE == FFN_UP_SWIGLU ? c.I : 128;
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.h = static_cast<__nv_bfloat16*>(h);
+  a.h = static_cast<float*>(h);
+  if (!aligned(h, 32)) return fail("expert_ffn: h must start on a 32-byte boundary");
   // rows whose starts, and the starts of their up halves, all lie on 32-byte boundaries
   a.wide = (MODE == FFN_DOWN || MODE == FFN_DROWS ? N : c.I) % 16 == 0 && aligned(out, 32);
-  a.wide_h = c.I % 16 == 0 && aligned(h, 32);
   a.status = c.dev->status;
   a.limit_ns = kOpWaitNs;
   const int feats = MODE == FFN_UP_SWIGLU ? N / 2 : N;

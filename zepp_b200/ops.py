@@ -17,6 +17,7 @@ leaves that no graph outside of it still holds (torch runs a leaf's accumulation
 import ctypes
 from typing import NamedTuple
 
+import numpy as np
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -45,6 +46,8 @@ _ARGS = {
     "zepp_op_grad_norm": (_P, _P, _P, _I, _D, _P, _P, _P),
     "zepp_op_status": (_P, _P),
 }
+# a small call is bound by the host: these two cost a tenth of torch.cuda.current_device() and current_stream()
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _SIZES = ("zepp_op_sort_ws_ints", "zepp_op_grad_norm_ws_bytes")
 _fns = {}
 
@@ -65,11 +68,12 @@ def _refuse(what):
 
 def _call(name, device, *args):
     """One entry point on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        rc = _fn(name)(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == _current_device():
+        rc = _fn(name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = _fn(name)(*args, torch.cuda.current_stream().cuda_stream)
+            rc = _fn(name)(*args, _raw_stream(index))
     if rc:
         check(rc)
 
@@ -265,8 +269,9 @@ def _ffn(rows, offsets, w1, w2, act, keep):
     n, H = rows.shape
     G, f1 = w1.shape[:2]
     I = w2.shape[2]
-    new = lambda c: torch.empty((n, c), dtype=torch.bfloat16, device=rows.device)  # noqa: E731
-    y, a, h = new(H), new(I), new(f1) if keep else None
+    y = torch.empty_like(rows)
+    a = torch.empty((n, I), dtype=torch.bfloat16, device=rows.device)
+    h = torch.empty((n, f1), dtype=torch.float32, device=rows.device) if keep else None
     _call("zepp_op_expert_ffn", rows.device, rows.data_ptr(), n, offsets.data_ptr(), G, H, I, act, w1.data_ptr(), w2.data_ptr(),
           a.data_ptr(), _ptr(h), y.data_ptr())
     return y, a, h
@@ -338,25 +343,26 @@ def _norm(tensors, max_norm):
     if not tensors:
         _refuse("no tensors")
     device = tensors[0].device
-    types = [_TYPES.get(t.dtype, -1) for t in tensors]
-    if device.type != "cuda" or min(types) < 0 or any(t.device != device for t in tensors):
+    types = [_TYPES.get(t.dtype, 255) for t in tensors]
+    if device.type != "cuda" or max(types) > 2 or set(map(torch.Tensor.get_device, tensors)) != {device.index}:
         _refuse("CUDA tensors of one device, of float32, bfloat16 or float16")
-    ptrs = [t.data_ptr() for t in tensors]
-    sizes = [t.numel() for t in tensors]
-    if not all(t.is_contiguous() or _is_dense(t) for t in tensors if t.numel()):
+    if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.is_contiguous() or _is_dense(t) for t in tensors):
         _refuse("tensors whose elements lie without gaps and only once in memory")
-    if max_norm >= 0:
-        last = 0
-        for p, n, ty in sorted(zip(ptrs, sizes, types)):
-            if n:
-                if p < last:
-                    _refuse("tensors that do not overlap (one is given twice?)")
-                last = p + n * (2 if ty else 4)
     n = len(tensors)
+    ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.uint64, n)
+    sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
+    types = np.array(types, np.uint8)
+    if max_norm >= 0:
+        some = sizes > 0
+        first = ptrs[some]
+        last = first + (sizes[some] * np.where(types[some] == 0, 4, 2)).astype(np.uint64)
+        order = first.argsort()
+        if (first[order[1:]] < last[order[:-1]]).any():
+            _refuse("tensors that do not overlap (one is given twice?)")
     out = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(_fn("zepp_op_grad_norm_ws_bytes")(n), dtype=torch.uint8, device=device)
-    _call("zepp_op_grad_norm", device, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*sizes), bytes(types), n,
-          max_norm, out.data_ptr(), ws.data_ptr())
+    _call("zepp_op_grad_norm", device, ptrs.ctypes.data, sizes.ctypes.data, types.ctypes.data, n, max_norm, out.data_ptr(),
+          ws.data_ptr())
     return out
 
 
