@@ -688,3 +688,33 @@ def test_sort_of_many_copies_passes_32_bit_offsets():
     assert torch.equal(rows[plan.position[some].long()], x[some][:, None, :].expand(-1, K, -1))
     y = zb.unsort_tokens(rows, plan, torch.full((T, K), 0.125, device="cuda"))
     assert torch.equal(y, x)
+
+
+@pytest.mark.parametrize("T, K, H, dtype", [(700, 8, 2048, torch.bfloat16), (613, 3, 1032, torch.float32), (2500, 11, 1160, torch.float16), (601, 20, 7168, torch.bfloat16)])
+def test_unsort_of_many_long_rows(T, K, H, dtype):
+    """Long rows in large numbers go through shared memory in pieces: whole and ragged last pieces, more copies than eight."""
+    g = gen(T)
+    ids = torch.randint(-2, 50, (T, K), generator=g, device="cuda", dtype=torch.int32)
+    ids[5] = -1
+    _, plan = zb.sort_tokens(randn((T, 8), g), ids, 50)
+    r, w = randn((T * K, H), g, dtype).requires_grad_(True), randn((T, K), g).requires_grad_(True)
+    dy = randn((T, H), g, dtype)
+    y = zb.unsort_tokens(r, plan, w)
+    dr, dw = torch.autograd.grad(y, (r, w), dy)
+    took = (plan.position >= 0)
+    pos = plan.position.clamp_min(0).long()
+    y64, size, dw64, dsize = (torch.zeros((T, n), dtype=torch.float64, device="cuda") for n in (H, H, K, K))
+    dr64 = torch.zeros((T * K, H), dtype=torch.float64, device="cuda")
+    for k in range(K):
+        row = r.detach()[pos[:, k]].double() * took[:, k, None]
+        y64 += row * w.detach()[:, k, None].double()
+        size += (row * w.detach()[:, k, None].double()).abs()
+        dw64[:, k], dsize[:, k] = (row * dy.double()).sum(1), (row * dy.double()).abs().sum(1)
+        t = took[:, k].nonzero()[:, 0]
+        dr64[pos[t, k]] = w.detach()[t, k, None].double() * dy[t].double()
+    within(y, y64, HALF[dtype] * y64.abs() + 2 * K * U * size + torch.finfo(dtype).tiny, "y")
+    within(dr, dr64, (HALF[dtype] + 2 * U) * dr64.abs() + torch.finfo(dtype).tiny, "drows")
+    within(dw, dw64, (H / 32 + 8 + 13) * U * dsize + 1e-30, "dweights")
+    assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r, plan, w.detach()), r, dy)[0], dr)       # without dweights
+    assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r.detach(), plan, w), w, dy)[0], dw)       # without drows
+    ops.check_waits()

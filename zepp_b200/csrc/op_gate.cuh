@@ -9,9 +9,10 @@
 // places, and a NaN anywhere in a row makes its weights NaN.
 //
 // A warp owns a row and holds it in registers, so the logits are read once: element (j / 4) * 128 + lane * 4 + j % 4 for
-// register j, four neighbours per access.  Each of the k rounds takes the maximum of an order-preserving integer key with
-// redux.sync and the lowest index that has it with a second one; only the winner's lane looks through its registers
-// again.  Bound by instruction issue from about 8 rounds on, by the bytes of the logits below that.
+// register j, four neighbours per access.  The (k + 1)-th largest of the 32 lanes' largest keys (order-preserving
+// integers, redux.sync) is a bound that hardly more than k keys reach; those few are put together, one per lane, and each
+// counts the ones before it (up to k = 20 or so they are fewer than 32; a row with more goes through 64 bits).  That is about 20 instructions per place, where k rounds of a maximum over all registers took
+// 200 (16381 rows of 384 bf16 logits with a bias: 30 us against 45 us).  Bound by instruction issue.
 #pragma once
 #include "op_common.cuh"
 
@@ -44,43 +45,52 @@ __device__ __forceinline__ unsigned gate_key(float v) {      // larger key <=> l
 __device__ __forceinline__ float gate_value(unsigned key) {
   return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
 }
-__device__ __forceinline__ int gate_index(int lane, int j) { return (j >> 2) * 128 + lane * 4 + (j & 3); }
+// The element that register j of a lane holds: four neighbours, 128 elements further the next four.  Up to 64 experts
+// (NPL = 4) the lanes take every 32nd element instead, so that each has some.
+template <int NPL>
+__device__ __forceinline__ int gate_index(int G, int lane, int j) {
+  if (NPL == 4 && G <= 64) return j * 32 + lane;
+  return (j >> 2) * 128 + lane * 4 + (j & 3);
+}
 
 template <typename T, int NPL>
 __device__ __forceinline__ void gate_load(const T* row, int G, int lane, bool vec, float (&v)[NPL], float fill) {
+  if (vec && G > 64) {
 #pragma unroll
-  for (int q = 0; q < NPL / 4; ++q) {
-    const int i = gate_index(lane, 4 * q);
-    if (vec) {
-      if (i < G) {
-        const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(row + i);
+    for (int q = 0; q < NPL / 4; ++q) {
+      const int i = gate_index<NPL>(G, lane, 4 * q);
+      Pack<T, 4> p;
+      if (i < G) p = *reinterpret_cast<const Pack<T, 4>*>(row + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = to_f32<T>(p.v[e]);
-      } else {
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = i < G ? to_f32<T>(p.v[e]) : fill;
+    }
+  } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = fill;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * q + e] = i + e < G ? to_f32<T>(row[i + e]) : fill;
+    for (int j = 0; j < NPL; ++j) {
+      const int i = gate_index<NPL>(G, lane, j);
+      v[j] = i < G ? to_f32<T>(row[i]) : fill;
     }
   }
 }
 
 __device__ __forceinline__ float sigmoid_f32(float l) { return 1.0f / (1.0f + expf(-l)); }
 
-// The choice by s + bias in 64 bits, for rows where two neighbours of the order lie within the rounding of the 32-bit
-// values: lane j < k returns its choice, -1 where none is left.
-template <int NPL>
-__device__ __noinline__ int gate_choose_f64(const float (&l)[NPL], const float* bias, int G, int k, int lane) {
+// The choice by the scores in 64 bits, straight from the row: for rows where the balanced scores of two neighbours of the
+// order lie within the rounding of the 32-bit values, and for rows with too many equal values to sort them in one warp.
+// Lane j < k returns its choice, -1 where none is left.
+template <typename T, int NPL>
+__device__ __noinline__ int gate_choose_f64(const T* row, const float* bias, int G, int k, int lane) {
   double key[NPL];
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
-    const int i = gate_index(lane, j);
+    const int i = gate_index<NPL>(G, lane, j);
     key[j] = -INFINITY;
-    if (i < G && l[j] > -INFINITY) {
-      const double v = 1.0 / (1.0 + exp(-(double)l[j])) + (double)bias[i];
-      if (v > -INFINITY) key[j] = v;                 // false for NaN
+    if (i < G) {
+      const float l = to_f32<T>(row[i]);
+      if (l > -INFINITY) {
+        const double v = bias != nullptr ? 1.0 / (1.0 + exp(-(double)l)) + (double)bias[i] : (double)l;
+        if (v > -INFINITY) key[j] = v;                 // false for NaN
+      }
     }
   }
   int mine = -1;
@@ -89,7 +99,7 @@ __device__ __noinline__ int gate_choose_f64(const float (&l)[NPL], const float* 
     int at = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
+      if (key[j] > best) { best = key[j]; at = gate_index<NPL>(G, lane, j); }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const double ob = __shfl_xor_sync(0xffffffffu, best, o);
@@ -100,65 +110,87 @@ __device__ __noinline__ int gate_choose_f64(const float (&l)[NPL], const float* 
     if (lane == r) mine = at;
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (gate_index(lane, j) == at) key[j] = -INFINITY;
+      if (gate_index<NPL>(G, lane, j) == at) key[j] = -INFINITY;
   }
   return mine;
 }
 
 template <typename T, int NPL>
 __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a) {
+  __shared__ uint2 s_cand[kGateWarps][32];           // (key, index) of the row's candidates
+  __shared__ uint2 s_order[kGateWarps][34];          // the first k + 1 of them in order
   const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * kGateWarps + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5;
+  const int G = a.G;
+  const long long row = (long long)blockIdx.x * kGateWarps + warp;
   if (row >= a.T) return;
   const T* src = static_cast<const T*>(a.logits) + row * a.G;
   float l[NPL];
   gate_load<T, NPL>(src, a.G, lane, a.vec, l, -INFINITY);
   unsigned key[NPL];
+  unsigned best = 0;
   bool nan = false;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
     nan |= l[j] != l[j];
     float v = l[j];
     if (a.bias != nullptr) {
-      const int i = gate_index(lane, j);
-      v = l[j] > -INFINITY ? sigmoid_f32(l[j]) + a.bias[i < a.G ? i : 0] : -INFINITY;
+      const int i = gate_index<NPL>(G, lane, j);
+      v = l[j] > -INFINITY ? __fdividef(1.0f, 1.0f + __expf(-l[j])) + a.bias[i < a.G ? i : 0] : -INFINITY;
     }
     key[j] = gate_key(v);
+    best = max(best, key[j]);
   }
   nan = __any_sync(0xffffffffu, nan);
 
-  int mine = -1;                 // lane j < k: the j-th choice
-  unsigned top = 0, last = 0;    // the largest key of the row; the key of the round before
-  bool doubt = false;
-  unsigned best = 0;
-  int at = 0;                    // this lane's largest key and the lowest index that has it
+  // A bound that at least k + 1 keys reach (if the row has so many): the (k + 1)-th largest of the lanes' largest keys.
+  // Equal ones leave together, which only lowers it.
+  const unsigned top = __reduce_max_sync(0xffffffffu, best);
+  unsigned bound = top;
+  for (int r = 0; r < a.k; ++r) {
+    if (best == bound) best = 0;
+    bound = __reduce_max_sync(0xffffffffu, best);
+  }
+  if (bound == 0) bound = 1;                         // fewer lanes than that: every key that can be chosen
+  int cnt = 0;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j)
-    if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
-  const int rounds = a.bias != nullptr ? a.k + 1 : a.k;      // one more shows how far behind the next expert is
-  for (int r = 0; r < rounds; ++r) {
-    const unsigned m = __reduce_max_sync(0xffffffffu, best);
-    if (m == 0u) break;
-    const int i = (int)__reduce_min_sync(0xffffffffu, best == m ? (unsigned)at : 0x7fffffffu);
-    if (r == 0) top = m;
-    if (a.bias != nullptr) {
-      // the 32-bit score is off by at most 2.5 units of 2^-24 for the exponential, one each for the sum, the quotient
-      // and the addition of the bias (relative to |s + b|): 4e-7 covers both sides of a comparison of s <= 1
-      const float v = gate_value(m);
-      if (r > 0 && gate_value(last) - v <= 8e-7f + 2.4e-7f * fabsf(v)) doubt = true;
-      last = m;
+  for (int j = 0; j < NPL; ++j) cnt += key[j] >= bound ? 1 : 0;
+  int at = cnt;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += u;
+  }
+  const int n = __shfl_sync(0xffffffffu, at, 31);
+  int mine = -1;                                     // lane j < k: the j-th choice
+  bool again = n > 32;
+  if (!again) {
+    at -= cnt;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (key[j] >= bound) s_cand[warp][at++] = make_uint2(key[j], (unsigned)gate_index<NPL>(G, lane, j));
+    if (lane < a.k + 1) s_order[warp][lane] = make_uint2(0u, 0xffffffffu);
+    if (lane == 0) s_order[warp][a.k] = make_uint2(0u, 0xffffffffu);
+    __syncwarp();
+    const uint2 me = s_cand[warp][lane];             // beyond n: never used
+    int rank = 0;
+    for (int c = 0; c < n; ++c) {
+      const uint2 o = s_cand[warp][c];
+      rank += o.x > me.x || (o.x == me.x && o.y < me.y) ? 1 : 0;
     }
-    if (lane == r && r < a.k) mine = i;
-    if (at == i && best == m) {
-      best = 0;
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) {
-        if (gate_index(lane, j) == i) key[j] = 0;
-        if (key[j] > best) { best = key[j]; at = gate_index(lane, j); }
-      }
+    if (lane < n && rank <= a.k) s_order[warp][rank] = me;
+    __syncwarp();
+    const uint2 chosen = s_order[warp][lane < a.k ? lane : a.k];
+    if (lane < a.k) mine = (int)chosen.y;
+    if (a.bias != nullptr) {
+      // A 32-bit score is off by at most 1.6e-6 s (1 - s) <= 4e-7 for the exponential (its argument is rounded, |l| <= 16
+      // where s (1 - s) matters), 1.2e-7 for the quotient and half a step of s + bias; twice that for two of them.
+      const uint2 next = s_order[warp][lane < a.k ? lane + 1 : a.k];
+      const float v = gate_value(chosen.x), w = gate_value(next.x);
+      again = __any_sync(0xffffffffu, lane < a.k && next.x != 0u && v - w <= 2e-6f + 2.4e-7f * fabsf(v));
     }
   }
-  if (doubt) mine = gate_choose_f64<NPL>(l, a.bias, a.G, a.k, lane);
+  if (again) mine = gate_choose_f64<T, NPL>(src, a.bias, a.G, a.k, lane);
 
   const float lc = mine >= 0 ? to_f32<T>(src[mine]) : 0.0f;
   float w = 0.0f;
@@ -174,7 +206,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a)
     } else {
       sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) sum += expf(l[j] - mx);
+      for (int j = 0; j < NPL; ++j) sum += __expf(l[j] - mx);
       sum = warp_sum(sum);
     }
     if (mine >= 0) w /= sum;
@@ -197,6 +229,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_grad_kernel(const GateAr
   extern __shared__ __align__(16) unsigned char gate_rows[];       // kGateWarps rows of G elements, 16-byte multiples
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
+  const int G = a.G;
   const long long row = (long long)blockIdx.x * kGateWarps + warp;
   if (row >= a.T) return;
   const T* src = static_cast<const T*>(a.logits) + row * a.G;
@@ -257,7 +290,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_grad_kernel(const GateAr
   T* st = reinterpret_cast<T*>(gate_rows) + (size_t)warp * ((a.G + 7) / 8 * 8);
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
-    const int i = gate_index(lane, j);
+    const int i = gate_index<NPL>(G, lane, j);
     if (i < a.G) st[i] = from_f32<T>(p[j]);
   }
   __syncwarp();

@@ -7,7 +7,7 @@
 // last chunk first, while the end of what the first launch read is still in L2.  Bound by HBM: one read, and one read and
 // one write where the norm is over the limit; with c = 1 nothing is touched.  Inside a chunk a thread adds at most
 // 64 squares in 32 bits, then carries on in 64; a chunk sum that left the range in which that is exact enough (values
-// beyond 1e19 or below 1e-16) is formed again in 64 bits from the registers.
+// beyond 1e19 or below 1e-16) is formed again in 64 bits.
 #pragma once
 #include "op_common.cuh"
 
@@ -29,34 +29,6 @@ struct NormTable {
   int count;
 };
 
-template <typename T>
-__device__ __forceinline__ float norm_chunk_sum(const uint4 (&v)[kNormVecs], double& wide) {
-  constexpr int E = 16 / (int)sizeof(T);
-  float s = 0.0f;
-  unsigned any = 0;
-#pragma unroll
-  for (int q = 0; q < kNormVecs; ++q) {
-    const T* e = reinterpret_cast<const T*>(&v[q]);
-    float sq = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) { const float x = to_f32<T>(e[i]); sq = fmaf(x, x, sq); }
-    s += sq;
-    any |= v[q].x | v[q].y | v[q].z | v[q].w;
-  }
-  if (any != 0u && !(s > 1e-30f && s < INFINITY)) {
-    wide = 0.0;
-#pragma unroll 1
-    for (int q = 0; q < kNormVecs; ++q) {
-      const T* e = reinterpret_cast<const T*>(&v[q]);
-#pragma unroll
-      for (int i = 0; i < E; ++i) { const double x = (double)to_f32<T>(e[i]); wide = fma(x, x, wide); }
-    }
-    return 0.0f;
-  }
-  wide = 0.0;
-  return s;
-}
-
 // this thread's vectors of chunk `c` of a tensor; elements outside it read as zero
 template <typename T>
 __device__ __forceinline__ void norm_load(const T* base, long long head, long long end, long long first, uint4 (&v)[kNormVecs]) {
@@ -74,6 +46,42 @@ __device__ __forceinline__ void norm_load(const T* base, long long head, long lo
         if (e0 + i >= head && e0 + i < end) e[i] = base[e0 + i];
     }
   }
+}
+
+// this thread's elements of a chunk once more, in 64 bits
+template <typename T>
+__device__ __noinline__ double norm_chunk_wide(const T* base, long long head, long long end, long long first) {
+  constexpr int E = 16 / (int)sizeof(T);
+  double s = 0.0;
+  for (int q = 0; q < kNormVecs; ++q) {
+    const long long e0 = first + (long long)(q * kNormThreads + threadIdx.x) * E;
+    for (int i = 0; i < E; ++i)
+      if (e0 + i >= head && e0 + i < end) {
+        const double x = (double)to_f32<T>(base[e0 + i]);
+        s = fma(x, x, s);
+      }
+  }
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ double norm_chunk_sum(const T* base, long long head, long long end, long long first) {
+  constexpr int E = 16 / (int)sizeof(T);
+  uint4 v[kNormVecs];
+  norm_load<T>(base, head, end, first, v);
+  float s = 0.0f;
+  unsigned any = 0;
+#pragma unroll
+  for (int q = 0; q < kNormVecs; ++q) {
+    const T* e = reinterpret_cast<const T*>(&v[q]);
+    float sq = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { const float x = to_f32<T>(e[i]); sq = fmaf(x, x, sq); }
+    s += sq;
+    any |= v[q].x | v[q].y | v[q].z | v[q].w;
+  }
+  if (any != 0u && !(s > 1e-30f && s < INFINITY)) return norm_chunk_wide<T>(base, head, end, first);
+  return (double)s;
 }
 
 template <typename T>
@@ -125,20 +133,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_partials_kernel(const __gri
   for (int c = blockIdx.x; c < t.chunk0[t.count]; c += gridDim.x) {
     const int k = norm_tensor_of(t, c);
     const long long bytes = (long long)(c - t.chunk0[k]) * kNormChunkBytes;
-    uint4 v[kNormVecs];
-    double wide = 0.0;
-    float s;
-    if (t.type[k] == OP_F32) {
-      norm_load<float>(reinterpret_cast<const float*>(t.base[k]), t.head[k], t.end[k], bytes / 4, v);
-      s = norm_chunk_sum<float>(v, wide);
-    } else if (t.type[k] == OP_BF16) {
-      norm_load<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(t.base[k]), t.head[k], t.end[k], bytes / 2, v);
-      s = norm_chunk_sum<__nv_bfloat16>(v, wide);
-    } else {
-      norm_load<__half>(reinterpret_cast<const __half*>(t.base[k]), t.head[k], t.end[k], bytes / 2, v);
-      s = norm_chunk_sum<__half>(v, wide);
-    }
-    sum += (double)s + wide;
+    if (t.type[k] == OP_F32)
+      sum += norm_chunk_sum<float>(reinterpret_cast<const float*>(t.base[k]), t.head[k], t.end[k], bytes / 4);
+    else if (t.type[k] == OP_BF16)
+      sum += norm_chunk_sum<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(t.base[k]), t.head[k], t.end[k], bytes / 2);
+    else
+      sum += norm_chunk_sum<__half>(reinterpret_cast<const __half*>(t.base[k]), t.head[k], t.end[k], bytes / 2);
   }
   sum = norm_block_sum(sum);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;

@@ -140,18 +140,25 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(const SortArgs 
     if (tid < m) a.position[tb * a.K + tid] = pos;
     __syncthreads();
     if (g >= 0) atomicMax(&next[g], pos + 1);
-    // the rows: 32 neighbouring vectors of a token per warp and step
+    // the rows: 32 neighbouring vectors of a token per warp and step, four steps' loads in flight
     const int lines = (int)((vecs + 31) / 32);
-    for (int u = warp; u < tokens * lines; u += kSortThreads / 32) {
-      const int t = u / lines;
-      const int v = (u - t * lines) * 32 + lane;
-      if (v < vecs) {
-        const V val = reinterpret_cast<const V*>(a.x + (tb + t) * a.row_bytes)[v];
-        for (int k = 0; k < a.K; ++k) {
-          const int p = s_pos[t * a.K + k];
-          if (p >= 0) reinterpret_cast<V*>(a.rows + (long long)p * a.row_bytes)[v] = val;
-        }
+    for (int u0 = warp; u0 < tokens * lines; u0 += 4 * (kSortThreads / 32)) {
+      V val[4];
+      int t[4], v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int u = u0 + q * (kSortThreads / 32);
+        t[q] = u / lines;
+        v[q] = u < tokens * lines ? (u - t[q] * lines) * 32 + lane : (int)vecs;
+        if (v[q] < vecs) val[q] = reinterpret_cast<const V*>(a.x + (tb + t[q]) * a.row_bytes)[v[q]];
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (v[q] < vecs)
+          for (int k = 0; k < a.K; ++k) {
+            const int p = s_pos[t[q] * a.K + k];
+            if (p >= 0) reinterpret_cast<V*>(a.rows + (long long)p * a.row_bytes)[v[q]] = val[q];
+          }
     }
     __syncthreads();
   }
@@ -161,6 +168,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_rows_kernel(const SortArgs 
 }
 
 constexpr int kUnsortThreads = 256;
+constexpr int kUnsortGradThreads = 128;
 
 struct UnsortArgs {
   const void* rows;        // [N, H]
@@ -182,65 +190,84 @@ __device__ __forceinline__ int unsort_position(const UnsortArgs& a, long long i)
   return p < a.N ? p : -1;
 }
 
-// E elements of a row per thread and step; blockIdx.x = token, blockIdx.y = part of the row
-template <typename T, int E>
+// A thread adds up U vectors of E elements (kUnsortThreads vectors apart) of a token's row, KU rows at a time in flight;
+// blockIdx.x = token, blockIdx.y = part of the row.
+template <typename T, int E, int U, int KU>
 __global__ void __launch_bounds__(kUnsortThreads) unsort_kernel(const UnsortArgs a) {
   typedef Pack<T, E> V;
   const long long t = blockIdx.x;
-  const long long vecs = a.H / E;
-  const long long v = (long long)blockIdx.y * kUnsortThreads + threadIdx.x;
-  if (v >= vecs) return;
-  float acc[E];
+  const int vecs = (int)(a.H / E);
+  const int v0 = blockIdx.y * (kUnsortThreads * U) + threadIdx.x;
+  float acc[U][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-  for (int k0 = 0; k0 < a.K; k0 += 4) {                  // four rows in flight
-    V r[4];
-    float w[4];
-    bool there[4];
+  for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int e = 0; e < E; ++e) acc[u][e] = 0.0f;
+  for (int k0 = 0; k0 < a.K; k0 += KU) {
+    V r[KU][U];
+    float w[KU];
+    int p[KU];
+#pragma unroll
+    for (int q = 0; q < KU; ++q) {
       const int k = k0 + q;
-      const int p = k < a.K ? unsort_position(a, t * a.K + k) : -1;
-      there[q] = p >= 0;
-      if (there[q]) {
-        w[q] = a.weights != nullptr ? a.weights[t * a.K + k] : 1.0f;
-        r[q] = reinterpret_cast<const V*>(static_cast<const T*>(a.rows) + (long long)p * a.H)[v];
-      }
+      p[q] = k < a.K ? unsort_position(a, t * a.K + k) : -1;
+      w[q] = k < a.K && a.weights != nullptr ? a.weights[t * a.K + k] : 1.0f;
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (there[q]) {
+    for (int q = 0; q < KU; ++q)
+      if (p[q] >= 0) {
+        const V* src = reinterpret_cast<const V*>(static_cast<const T*>(a.rows) + (long long)p[q] * a.H);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w[q], to_f32<T>(r[q].v[e]), acc[e]);
+        for (int u = 0; u < U; ++u)
+          if (v0 + u * kUnsortThreads < vecs) r[q][u] = src[v0 + u * kUnsortThreads];
+      }
+#pragma unroll
+    for (int q = 0; q < KU; ++q)
+      if (p[q] >= 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[u][e] = fmaf(w[q], to_f32<T>(r[q][u].v[e]), acc[u][e]);
       }
   }
-  V out;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out.v[e] = from_f32<T>(acc[e]);
-  reinterpret_cast<V*>(static_cast<T*>(a.y) + t * a.H)[v] = out;
+  for (int u = 0; u < U; ++u)
+    if (v0 + u * kUnsortThreads < vecs) {
+      V out;
+#pragma unroll
+      for (int e = 0; e < E; ++e) out.v[e] = from_f32<T>(acc[u][e]);
+      reinterpret_cast<V*>(static_cast<T*>(a.y) + t * a.H)[v0 + u * kUnsortThreads] = out;
+    }
 }
 
-// a block owns a token: dy is read once for eight copies, each row once
+// `wpt` warps of a block own a token: dy is read once for eight copies, each row once.  With one warp per token nothing in
+// the block waits for anything else.
 template <typename T, int E>
-__global__ void __launch_bounds__(kUnsortThreads) unsort_grad_kernel(const UnsortArgs a) {
+__global__ void __launch_bounds__(kUnsortGradThreads) unsort_grad_kernel(const UnsortArgs a, int wpt) {
   typedef Pack<T, E> V;
   constexpr int KB = 8;
-  __shared__ float s_dot[kUnsortThreads / 32][KB];
-  const long long vecs = a.H / E;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (long long t = blockIdx.x; t < a.T; t += gridDim.x) {
-    const V* dy = reinterpret_cast<const V*>(static_cast<const T*>(a.dy) + t * a.H);
+  __shared__ float s_dot[2][kUnsortGradThreads / 32][KB];
+  const int vecs = (int)(a.H / E);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per_block = kUnsortGradThreads / 32 / wpt;
+  const int sub = warp % wpt, first = warp - sub;        // this warp among its token's, and the first of them
+  int flip = 0;
+  // a block's warps go round together (the barrier below), those behind the last token without one
+  for (long long t0 = (long long)blockIdx.x * per_block; t0 < a.T; t0 += (long long)gridDim.x * per_block) {
+    const long long t = t0 + warp / wpt;
+    const bool real = t < a.T;
+    const V* dy = reinterpret_cast<const V*>(static_cast<const T*>(a.dy) + (real ? t : 0) * a.H);
     for (int k0 = 0; k0 < a.K; k0 += KB) {
       int p[KB];
       float w[KB], dot[KB];
 #pragma unroll
       for (int q = 0; q < KB; ++q) {
         const int k = k0 + q;
-        p[q] = k < a.K ? unsort_position(a, t * a.K + k) : -1;
-        w[q] = p[q] >= 0 && a.weights != nullptr ? a.weights[t * a.K + k] : 1.0f;
+        p[q] = real && k < a.K ? unsort_position(a, t * a.K + k) : -1;
+        w[q] = real && k < a.K && a.weights != nullptr ? a.weights[t * a.K + k] : 1.0f;
         dot[q] = 0.0f;
       }
-      for (long long v = tid; v < vecs; v += blockDim.x) {
+      for (int v = sub * 32 + lane; real && v < vecs; v += wpt * 32) {
         const V d = dy[v];
         if (a.dweights != nullptr) {
           V r[KB];
@@ -266,26 +293,257 @@ __global__ void __launch_bounds__(kUnsortThreads) unsort_grad_kernel(const Unsor
         }
       }
       if (a.dweights != nullptr) {
+        float mine = 0.0f;                               // lane q: the sum for copy k0 + q
 #pragma unroll
         for (int q = 0; q < KB; ++q) {
           const float s = warp_sum(dot[q]);
-          if (lane == 0) s_dot[warp][q] = s;
+          if (lane == q) mine = p[q] >= 0 ? s : 0.0f;
         }
-        __syncthreads();
-        if (tid < KB && k0 + tid < a.K) {
-          float s = 0.0f;
-          for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += s_dot[i][tid];
-          a.dweights[t * a.K + k0 + tid] = unsort_position(a, t * a.K + k0 + tid) >= 0 ? s : 0.0f;
+        if (wpt > 1) {
+          if (lane < KB) s_dot[flip][warp][lane] = mine;
+          __syncthreads();
+          if (sub == 0 && lane < KB)
+            for (int i = 1; i < wpt; ++i) mine += s_dot[flip][first + i][lane];
+          flip ^= 1;                                     // the other half is free: its readers passed this barrier
         }
-        __syncthreads();
+        if (sub == 0 && lane < KB && real && k0 + lane < a.K) a.dweights[t * a.K + k0 + lane] = mine;
       }
     }
   }
   if (a.drows != nullptr) {
-    long long first = *a.n_rows;
-    if (first < 0) first = 0;
-    for (long long p = first + blockIdx.x; p < a.N; p += gridDim.x)
-      for (long long v = tid; v < vecs; v += blockDim.x) reinterpret_cast<V*>(static_cast<T*>(a.drows) + p * a.H)[v] = V{};
+    long long begin = *a.n_rows;
+    if (begin < 0) begin = 0;
+    for (long long p = begin + blockIdx.x; p < a.N; p += gridDim.x)
+      for (int v = threadIdx.x; v < vecs; v += kUnsortGradThreads) reinterpret_cast<V*>(static_cast<T*>(a.drows) + p * a.H)[v] = V{};
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The same two for long rows in large numbers: one persistent block per SM, a warp that fetches pieces of the rows into a
+// ring of shared-memory stages with bulk copies, eight warps that add them up.  A stage holds one piece (kPieceBytes) of up
+// to eight copies' rows (GRAD: and of dy), so nearly 200 KB are in flight on every SM whatever the registers allow, and the
+// positions, the first link of each chain of loads, are read one stage ahead.
+// Steps of a block, `steps` in all per token: (piece, eight copies) with the copies inner, or GRAD: (eight copies, piece)
+// with the piece inner, so that a sum over k or over the row stays in registers.
+constexpr int kPieceBytes = 4096;
+constexpr int kPieceThreads = kPieceBytes / 16;         // consumers: a 16-byte vector each
+constexpr int kBulkThreads = 32 + kPieceThreads;
+constexpr int kBulkMaxStages = 16;
+constexpr int kBulkRingBytes = 48 * kPieceBytes;        // six stages, five with dy
+
+struct BulkArgs {
+  UnsortArgs u;
+  int pieces, chunks;         // of a row; of its copies, eight at a time
+  int stages, stage_bytes;
+  unsigned long long* status;
+  unsigned long long limit_ns;
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const BulkArgs b) {
+  constexpr int E = 16 / (int)sizeof(T);
+  typedef Pack<T, E> V;
+  const UnsortArgs& a = b.u;
+  extern __shared__ __align__(128) unsigned char bulk_ring[];
+  __shared__ __align__(8) uint64_t full[kBulkMaxStages], empty[kBulkMaxStages];
+  __shared__ int s_pos[kBulkMaxStages][8];
+  __shared__ float s_w[kBulkMaxStages][8];
+  __shared__ float s_dot[2][kPieceThreads / 32][8];
+  __shared__ int abort_flag;
+  volatile int* abortp = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < b.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kPieceThreads / 32);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // without GRAD a token's pieces are independent: blocks share them out
+  const int per_unit = GRAD ? b.pieces * b.chunks : b.chunks;
+  const int units = (int)(GRAD ? a.T : a.T * b.pieces);        // rows of 2 KB and more: far fewer than 2^31 fit the memory
+  const int mine = (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;      // gridDim.x <= units
+  const int total = mine * per_unit;
+  const long long row_bytes = a.H * (long long)sizeof(T);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- copies
+    // Positions and weights of four steps at a time (lane: step lane / 8, copy lane % 8), four steps ahead: they are the
+    // first link of every chain of loads, and one step ahead each stage still waited for most of their latency.
+    int unit = blockIdx.x, step = 0, stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    int p_next = -1, p_four = -1;
+    float w_next = 1.0f, w_four = 1.0f;
+    auto fetch = [&](int i) {
+      i += lane >> 3;
+      p_next = -1;
+      w_next = 1.0f;
+      if (i < total) {
+        const int u = (int)blockIdx.x + i / per_unit * (int)gridDim.x, st = i % per_unit;
+        const int k = (GRAD ? st / b.pieces : st) * 8 + (lane & 7);
+        const long long at = (long long)(GRAD ? u : u / b.pieces) * a.K + k;
+        if (k < a.K) {
+          p_next = unsort_position(a, at);
+          if (a.weights != nullptr) w_next = a.weights[at];
+        }
+      }
+    };
+    fetch(0);
+    for (int i = 0; i < total; ++i) {
+      if ((i & 3) == 0) {
+        p_four = p_next;
+        w_four = w_next;
+        fetch(i + 4);
+      }
+      const int from = (i & 3) * 8 + (lane & 7);
+      const int p_lane = __shfl_sync(0xffffffffu, p_four, from);
+      const int now_p = lane < 8 ? p_lane : -1;
+      const float now_w = __shfl_sync(0xffffffffu, w_four, from);
+      const int piece = GRAD ? step % b.pieces : unit % b.pieces;
+      const long long t = GRAD ? unit : unit / b.pieces;
+      const uint32_t at = (uint32_t)piece * kPieceBytes;
+      const uint32_t bytes = (uint32_t)min((long long)kPieceBytes, row_bytes - at);
+      if (++step == per_unit) { step = 0; unit += gridDim.x; }
+      const bool ok = mbar_wait_bounded(&empty[stage], phase ^ 1, abortp, b.limit_ns);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) {
+          record_timeout(b.status, WAIT_MBAR_EMPTY, t, i);
+          abort_flag = 1;
+        }
+        break;
+      }
+      if (lane < 8) {
+        s_pos[stage][lane] = now_p;
+        s_w[stage][lane] = now_w;
+      }
+      const bool rows = !GRAD || a.dweights != nullptr;
+      const uint32_t copies = rows ? __popc(__ballot_sync(0xffffffffu, now_p >= 0)) : 0u;
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(&full[stage], (copies + (GRAD ? 1u : 0u)) * bytes);
+      __syncwarp();
+      unsigned char* st = bulk_ring + (size_t)stage * b.stage_bytes;
+      if (rows && now_p >= 0)
+        bulk_load(st + lane * kPieceBytes, static_cast<const unsigned char*>(a.rows) + now_p * row_bytes + at, bytes, &full[stage]);
+      if (GRAD && lane == 8)
+        bulk_load(st + 8 * kPieceBytes, static_cast<const unsigned char*>(a.dy) + t * row_bytes + at, bytes, &full[stage]);
+      ++issued;
+      if (++stage == b.stages) { stage = 0; phase ^= 1; }
+    }
+    if (*abortp) {                                             // given up: the block stays until its copies have landed
+      int never = 0;
+      for (int i = issued > b.stages ? issued - b.stages : 0; i < issued; ++i)
+        mbar_wait_bounded(&full[i % b.stages], (uint32_t)(i / b.stages) & 1u, &never, b.limit_ns);
+    }
+  } else {
+    // ---------------------------------------------------------------- sums
+    const int v = threadIdx.x - 32;
+    int unit = blockIdx.x, step = 0, stage = 0, flip = 0;
+    uint32_t phase = 0;
+    float acc[GRAD ? 8 : E];
+#pragma unroll
+    for (int e = 0; e < (GRAD ? 8 : E); ++e) acc[e] = 0.0f;
+    for (int i = 0; i < total; ++i) {
+      const int piece = GRAD ? step % b.pieces : unit % b.pieces;
+      const int chunk = GRAD ? step / b.pieces : step;
+      const long long t = GRAD ? unit : unit / b.pieces;
+      const long long at = (long long)piece * kPieceBytes + v * 16;
+      const bool in = at < row_bytes;
+      const bool ok = mbar_wait_bounded(&full[stage], phase, abortp, b.limit_ns);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0 && !*abortp) record_timeout(b.status, WAIT_MBAR_FULL, t, i);
+        abort_flag = 1;
+        if (GRAD) asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");      // nobody is left waiting below
+        break;
+      }
+      const unsigned char* st = bulk_ring + (size_t)stage * b.stage_bytes + v * 16;
+      if (GRAD) {
+        if (in) {
+          const V d = *reinterpret_cast<const V*>(st + 8 * kPieceBytes);
+          float f[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = to_f32<T>(d.v[e]);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int p = s_pos[stage][q];
+            if (p >= 0) {
+              if (a.dweights != nullptr) {
+                const V r = *reinterpret_cast<const V*>(st + q * kPieceBytes);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[q] = fmaf(f[e], to_f32<T>(r.v[e]), acc[q]);
+              }
+              if (a.drows != nullptr) {
+                const float w = s_w[stage][q];
+                V o;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(w * f[e]);
+                *reinterpret_cast<V*>(static_cast<unsigned char*>(a.drows) + p * row_bytes + at) = o;
+              }
+            }
+          }
+        }
+      } else if (in) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (s_pos[stage][q] >= 0) {
+            const V r = *reinterpret_cast<const V*>(st + q * kPieceBytes);
+            const float w = s_w[stage][q];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, to_f32<T>(r.v[e]), acc[e]);
+          }
+      }
+      const int p_of_lane = GRAD && lane < 8 ? s_pos[stage][lane] : -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (++stage == b.stages) { stage = 0; phase ^= 1; }
+      if (GRAD) {
+        if (piece == b.pieces - 1) {                           // eight copies of a token are done
+          if (a.dweights != nullptr) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float s = warp_sum(acc[q]);
+              if (lane == q) s_dot[flip][warp - 1][q] = s;
+              acc[q] = 0.0f;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(kPieceThreads) : "memory");
+            if (__any_sync(0xffffffffu, *abortp)) {            // a warp that gave up has left: go too, and count for the next round
+              asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");
+              break;
+            }
+            if (warp == 1 && lane < 8 && chunk * 8 + lane < a.K) {
+              float s = 0.0f;
+              for (int w = 0; w < kPieceThreads / 32; ++w) s += s_dot[flip][w][lane];
+              a.dweights[t * a.K + chunk * 8 + lane] = p_of_lane >= 0 ? s : 0.0f;
+            }
+            flip ^= 1;                                         // the other half is free: its readers passed this barrier
+          }
+        }
+      } else if (chunk == b.chunks - 1) {
+        if (in) {
+          V o;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(acc[e]);
+          *reinterpret_cast<V*>(static_cast<unsigned char*>(a.y) + t * row_bytes + at) = o;
+        }
+#pragma unroll
+        for (int e = 0; e < (GRAD ? 8 : E); ++e) acc[e] = 0.0f;
+      }
+      if (++step == per_unit) { step = 0; unit += gridDim.x; }
+    }
+    if (GRAD && a.drows != nullptr) {
+      long long begin = *a.n_rows;
+      if (begin < 0) begin = 0;
+      for (long long p = begin + blockIdx.x; p < a.N; p += gridDim.x)
+        for (long long at = v * 16; at < row_bytes; at += kPieceBytes)
+          *reinterpret_cast<V*>(static_cast<unsigned char*>(a.drows) + p * row_bytes + at) = V{};
+    }
   }
 }
 

@@ -39,6 +39,13 @@ cudaError_t ffn_smem() {
   return cudaFuncSetAttribute(ffn_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmemBytes);
 }
 
+template <typename T>
+cudaError_t bulk_smem() {
+  cudaError_t e = cudaFuncSetAttribute(unsort_bulk_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkRingBytes);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(unsort_bulk_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkRingBytes);
+}
+
 // the current device's record; its first use sets kernel attributes and looks up the status block
 int op_device(OpDevice** out) {
   int dev = 0;
@@ -64,6 +71,9 @@ int op_device(OpDevice** out) {
     CU_OK(ffn_smem<FFN_DACT_GELU>());
     CU_OK(ffn_smem<FFN_DROWS>());
     CU_OK(ffn_smem<FFN_DWEIGHT>());
+    CU_OK(bulk_smem<float>());
+    CU_OK(bulk_smem<__nv_bfloat16>());
+    CU_OK(bulk_smem<__half>());
     d.ready = true;
   }
   *out = &d;
@@ -199,29 +209,56 @@ extern "C" int zepp_op_sort(const void* x, int dtype, int64_t T, int K, int64_t 
 }
 
 template <typename T, int E>
-static void unsort_launch(const UnsortArgs& a, bool grad, cudaStream_t s) {
+static void unsort_launch(const UnsortArgs& a, bool grad, int sms, cudaStream_t s) {
   const long long vecs = a.H / E;
   if (grad) {
-    // as many threads as a row has vectors, in whole warps
-    const int threads = (int)(vecs >= kUnsortThreads ? kUnsortThreads : (vecs + 31) / 32 * 32);
-    const long long blocks = a.T > 0 ? a.T : (a.N > 0 ? a.N : 1);
-    unsort_grad_kernel<T, E><<<(unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), threads, 0, s>>>(a);
-  } else {
-    unsort_kernel<T, E><<<dim3((unsigned)a.T, (unsigned)((vecs + kUnsortThreads - 1) / kUnsortThreads)), kUnsortThreads, 0, s>>>(a);
+    // a warp per token once that fills the machine (16 warps on every SM), else as many as a block has, as long as each
+    // has a vector for every lane
+    int wpt = 1;
+    while (wpt < kUnsortGradThreads / 32 && a.T * wpt < 16ll * sms && vecs > 32 * wpt) wpt *= 2;
+    const long long tokens = kUnsortGradThreads / 32 / wpt;
+    const long long blocks = (a.T + tokens - 1) / tokens;
+    unsort_grad_kernel<T, E><<<(unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), kUnsortGradThreads, 0, s>>>(a, wpt);
+  } else if (E > 1) {
+    const dim3 grid((unsigned)a.T, (unsigned)((vecs + kUnsortThreads - 1) / kUnsortThreads));
+    unsort_kernel<T, E, 1, 4><<<grid, kUnsortThreads, 0, s>>>(a);
+  } else {       // single elements: four per thread and row
+    const dim3 grid((unsigned)a.T, (unsigned)((vecs + 4 * kUnsortThreads - 1) / (4 * kUnsortThreads)));
+    unsort_kernel<T, E, E == 1 ? 4 : 1, 8><<<grid, kUnsortThreads, 0, s>>>(a);
   }
 }
+// pieces of rows through shared memory: worth it for rows of half a piece or more, once every block has several
+template <typename T, bool GRAD>
+static bool unsort_bulk(const UnsortArgs& a, const OpDevice* d, cudaStream_t s) {
+  const long long row_bytes = a.H * (long long)sizeof(T);
+  BulkArgs b{};
+  b.u = a;
+  b.pieces = (int)((row_bytes + kPieceBytes - 1) / kPieceBytes);
+  b.chunks = (a.K + 7) / 8;
+  const long long units = GRAD ? a.T : a.T * b.pieces;
+  if (row_bytes * 2 < kPieceBytes || units < 4ll * d->sms) return false;
+  b.stage_bytes = (GRAD ? 9 : 8) * kPieceBytes;
+  b.stages = kBulkRingBytes / b.stage_bytes;
+  b.status = d->status;
+  b.limit_ns = kOpWaitNs;
+  unsort_bulk_kernel<T, GRAD><<<d->sms, kBulkThreads, b.stages * b.stage_bytes, s>>>(b);
+  return true;
+}
 template <typename T>
-static void unsort_type(const UnsortArgs& a, bool grad, cudaStream_t s) {
+static void unsort_type(const UnsortArgs& a, bool grad, const OpDevice* d, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   const bool wide = a.H % E == 0 && aligned(a.rows, 16) && aligned(a.y, 16) && aligned(a.dy, 16) && aligned(a.drows, 16);
-  if (wide) unsort_launch<T, E>(a, grad, s);
-  else unsort_launch<T, 1>(a, grad, s);
+  if (wide && (grad ? unsort_bulk<T, true>(a, d, s) : unsort_bulk<T, false>(a, d, s))) return;
+  if (wide) unsort_launch<T, E>(a, grad, d->sms, s);
+  else unsort_launch<T, 1>(a, grad, d->sms, s);
 }
 static int unsort_run(const UnsortArgs& a, int dtype, bool grad, void* stream) {
+  OpDevice* d;
+  if (int rc = op_device(&d)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == OP_F32) unsort_type<float>(a, grad, s);
-  else if (dtype == OP_BF16) unsort_type<__nv_bfloat16>(a, grad, s);
-  else unsort_type<__half>(a, grad, s);
+  if (dtype == OP_F32) unsort_type<float>(a, grad, d, s);
+  else if (dtype == OP_BF16) unsort_type<__nv_bfloat16>(a, grad, d, s);
+  else unsort_type<__half>(a, grad, d, s);
   OP_LAUNCHED();
   return 0;
 }
