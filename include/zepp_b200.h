@@ -193,7 +193,7 @@ int zepp_op_unsort_grad(const void* dy_dev, const void* rows_dev, int dtype, int
 /* y [n, H] of rows [n, H] through expert e's w1 [G, f1, H], activation and w2 [G, H, I] for rows offsets[e] ..
  * offsets[e + 1] (offsets[0] counts as 0; y is zero behind the last expert's rows).  bf16; act as in zepp_layer_cfg;
  * f1 = 2 I (gate rows, then up rows) for swiglu, I for gelu; H and I multiples of 8, G <= 1024, tensors on 16-byte
- * boundaries.  a [n, I] takes the activations; h [n, f1] (fp32, on a 32-byte boundary) the
+ * boundaries.  a [n, I] takes the activations; h [n, f1] (fp32) the
  * products before them, or null: no gradient wanted. */
 int zepp_op_expert_ffn(const void* rows_dev, int64_t n, const int32_t* offsets_dev, int G, int H, int I, int act,
                        const void* w1_dev, const void* w2_dev, void* a_dev, void* h_dev, void* y_dev, void* stream);

@@ -34,9 +34,16 @@ struct OpDevice {
 OpDevice g_dev[kMaxDevices];
 std::mutex g_dev_mutex;
 
+// dynamic shared memory of the products: tables of G groups (behind at most 512 bytes of static shared memory), stages on
+// 1024-byte boundaries, staging of the epilogue warps
+size_t ffn_smem_bytes(int G, int stages) {
+  return (512 + 2 * sizeof(int) * (size_t)(G + 1) + 1023) / 1024 * 1024 + (size_t)stages * kFfnStageBytes + kFfnEpiWarps * kFfnStagingBytes;
+}
+constexpr int kFfnSmemLimit = 227 * 1024 - 512;
+
 template <int MODE>
 cudaError_t ffn_smem() {
-  return cudaFuncSetAttribute(ffn_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmemBytes);
+  return cudaFuncSetAttribute(ffn_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFfnSmemLimit);
 }
 
 template <typename T>
@@ -328,31 +335,35 @@ static int ffn_check(const char* what, int64_t n, int G, int H, int I, int act, 
   return 0;
 }
 
-// K-major rows [n, K] times the weights [G, wr, wc]
+// one launch of the products' kernel over at most `tiles` tiles
 template <int MODE>
-static int ffn_rows_launch(const FfnCall& c, const void* rows, int K, const void* w, int wr, int wc, int N, void* out, void* h) {
-  constexpr bool kBRows = MODE == FFN_UP_SWIGLU || MODE == FFN_UP_GELU || MODE == FFN_DOWN;
-  CUtensorMap a32, a64, a128, b;
-  if (int rc = ffn_map(&a32, rows, K, c.n, 0, 32)) return rc;
-  if (int rc = ffn_map(&a64, rows, K, c.n, 0, 64)) return rc;
-  if (int rc = ffn_map(&a128, rows, K, c.n, 0, 128)) return rc;
-  if (int rc = ffn_map(&b, w, wc, wr, c.G, kBRows ? 128 : 64)) return rc;
-  FfnArgs a{};
-  a.offsets = c.offsets; a.G = c.G; a.n = c.n; a.K = K; a.N = N;
-  a.feat = MODE == FFN_UP_SWIGLU ? 128 : 256;
-  a.up_offset = MODE == FFN_UP_SWIGLU ? c.I : 128;
-  a.out = static_cast<__nv_bfloat16*>(out);
-  a.h = static_cast<float*>(h);
-  if (!aligned(h, 32)) return fail("expert_ffn: h must start on a 32-byte boundary");
-  // rows whose starts, and the starts of their up halves, all lie on 32-byte boundaries
-  a.wide = (MODE == FFN_DOWN || MODE == FFN_DROWS ? N : c.I) % 16 == 0 && aligned(out, 32);
+static int ffn_launch(const FfnCall& c, int64_t tiles, const CUtensorMap& f, const CUtensorMap& r32, const CUtensorMap& r128, FfnArgs& a) {
+  a.offsets = c.offsets; a.G = c.G; a.n = c.n;
+  a.stages = kFfnMaxStages;
+  while (ffn_smem_bytes(c.G, a.stages) > (size_t)kFfnSmemLimit) --a.stages;      // the tables of 192 groups and more take one's place
   a.status = c.dev->status;
   a.limit_ns = kOpWaitNs;
-  const int feats = MODE == FFN_UP_SWIGLU ? N / 2 : N;
-  const int64_t tiles = (c.n / 128 + (c.n < c.G ? c.n : c.G)) * ((feats + a.feat - 1) / a.feat);
-  ffn_kernel<MODE><<<(unsigned)(tiles < c.dev->sms ? tiles : c.dev->sms), 192, kFfnSmemBytes, c.stream>>>(a32, a64, a128, b, a);
+  const int pairs = c.dev->sms / 2;
+  ffn_kernel<MODE><<<(unsigned)(tiles < pairs ? tiles : pairs) * 2, kFfnThreads, ffn_smem_bytes(c.G, a.stages), c.stream>>>(f, r32, r128, a);
   OP_LAUNCHED();
   return 0;
+}
+
+// K-major rows [n, K] times the weights [G, wr, wc]; N: features of the result (of each half, where it has two)
+template <int MODE>
+static int ffn_rows_launch(const FfnCall& c, const void* rows, int K, const void* w, int wr, int wc, int N, void* out, void* h) {
+  constexpr bool kWhole = MODE == FFN_UP_GELU || MODE == FFN_DOWN;       // 128 weight rows in one box
+  CUtensorMap r32, r128, f;
+  if (int rc = ffn_map(&r32, rows, K, c.n, 0, 32)) return rc;
+  if (int rc = ffn_map(&r128, rows, K, c.n, 0, 128)) return rc;
+  if (int rc = ffn_map(&f, w, wc, wr, c.G, kWhole ? 128 : 64)) return rc;
+  FfnArgs a{};
+  a.K = K; a.N = N;
+  a.feat = MODE == FFN_UP_SWIGLU ? 128 : 256;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.h = static_cast<float*>(h);
+  const int64_t tiles = (c.n / kFfnRows + (c.n < c.G ? c.n : c.G)) * ((N + a.feat - 1) / a.feat);
+  return ffn_launch<MODE>(c, tiles, f, r32, r128, a);
 }
 
 // dW [G, M, N] = p_e^T q_e over the rows of each expert
@@ -361,15 +372,10 @@ static int ffn_weight_launch(const FfnCall& c, const void* p, int M, const void*
   if (int rc = ffn_map(&mp, p, M, c.n, 0, 64)) return rc;
   if (int rc = ffn_map(&mq, q, N, c.n, 0, 64)) return rc;
   FfnArgs a{};
-  a.offsets = c.offsets; a.G = c.G; a.n = c.n; a.M = M; a.N = N; a.feat = 256;
+  a.M = M; a.N = N; a.feat = 256;
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.wide = N % 16 == 0 && aligned(out, 32);
-  a.status = c.dev->status;
-  a.limit_ns = kOpWaitNs;
-  const int64_t tiles = (int64_t)c.G * ((M + 127) / 128) * ((N + 255) / 256);
-  ffn_kernel<FFN_DWEIGHT><<<(unsigned)(tiles < c.dev->sms ? tiles : c.dev->sms), 192, kFfnSmemBytes, c.stream>>>(mp, mp, mp, mq, a);
-  OP_LAUNCHED();
-  return 0;
+  const int64_t tiles = (int64_t)c.G * ((M + 255) / 256) * ((N + kFfnRows - 1) / kFfnRows);
+  return ffn_launch<FFN_DWEIGHT>(c, tiles, mp, mq, mq, a);
 }
 
 extern "C" int zepp_op_expert_ffn(const void* rows, int64_t n, const int32_t* offsets, int G, int H, int I, int act,
@@ -379,7 +385,7 @@ extern "C" int zepp_op_expert_ffn(const void* rows, int64_t n, const int32_t* of
   FfnCall c{offsets, n, G, H, I, act, nullptr, static_cast<cudaStream_t>(stream)};
   if (int rc = op_device(&c.dev)) return rc;
   if (act) {
-    if (int rc = ffn_rows_launch<FFN_UP_SWIGLU>(c, rows, H, w1, 2 * I, H, 2 * I, a_out, h_out)) return rc;
+    if (int rc = ffn_rows_launch<FFN_UP_SWIGLU>(c, rows, H, w1, 2 * I, H, I, a_out, h_out)) return rc;
   } else {
     if (int rc = ffn_rows_launch<FFN_UP_GELU>(c, rows, H, w1, I, H, I, a_out, h_out)) return rc;
   }
