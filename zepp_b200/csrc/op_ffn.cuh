@@ -131,11 +131,6 @@ __device__ __forceinline__ void ffn_store8(float* out, const float (&x)[8]) {
   reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
   reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-__device__ __forceinline__ void ffn_load8(const float* in, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(in)[0], b = reinterpret_cast<const float4*>(in)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 
 // A warp's 32 rows (lanes) x 64 features (registers) as bf16 through its staging: 128 bytes a row, its 16-byte units
 // XOR-swizzled by the row, then eight lanes write a row's whole line.
@@ -164,31 +159,43 @@ __device__ __forceinline__ void ffn_put(uint4* stg, const uint32_t (&v)[32], con
   __syncwarp();
 }
 
+// h of eight features from f of row `row`, for the modes that read it: fetched before the accumulators are waited for
+struct FfnH {
+  float4 g[2], u[2];
+};
+template <int MODE>
+__device__ __forceinline__ void ffn_load_h(const FfnArgs& a, long long row, int f, FfnH& h) {
+  const float4* p = reinterpret_cast<const float4*>(a.h + row * (MODE == FFN_DACT_SWIGLU ? 2 : 1) * a.N + f);
+  h.g[0] = __ldg(p);
+  h.g[1] = __ldg(p + 1);
+  if (MODE == FFN_DACT_SWIGLU) {
+    const float4* q = reinterpret_cast<const float4*>(a.h + row * 2 * a.N + a.N + f);
+    h.u[0] = __ldg(q);
+    h.u[1] = __ldg(q + 1);
+  }
+}
+
 // Eight features from f of row `row`: what the mode makes of the accumulators x and stores.
 template <int MODE>
-__device__ __forceinline__ void ffn_finish8(const FfnArgs& a, long long row, int f, float (&x)[8]) {
+__device__ __forceinline__ void ffn_finish8(const FfnArgs& a, long long row, int f, float (&x)[8], const FfnH& h) {
+  const float* hg = reinterpret_cast<const float*>(h.g);
   if (MODE == FFN_DACT_SWIGLU) {
-    const float* h = a.h + row * 2 * a.N + f;
+    const float* hu = reinterpret_cast<const float*>(h.u);
     float g[8], u[8];
-    ffn_load8(h, g);
-    ffn_load8(h + a.N, u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float s = ffn_sigmoid(g[e]);
-      const float dg = x[e] * u[e] * s * (1.0f + g[e] * (1.0f - s));
-      u[e] = x[e] * g[e] * s;
-      g[e] = dg;
+      const float s = ffn_sigmoid(hg[e]);
+      g[e] = x[e] * hu[e] * s * (1.0f + hg[e] * (1.0f - s));
+      u[e] = x[e] * hg[e] * s;
     }
     ffn_store8(a.out + row * 2 * a.N + f, g);
     ffn_store8(a.out + row * 2 * a.N + a.N + f, u);
     return;
   }
   if (MODE == FFN_DACT_GELU) {
-    float h[8];
-    ffn_load8(a.h + row * a.N + f, h);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      x[e] *= 0.5f * (1.0f + erff(h[e] * 0.70710678118654752f)) + h[e] * 0.39894228040143268f * __expf(-0.5f * h[e] * h[e]);
+      x[e] *= 0.5f * (1.0f + erff(hg[e] * 0.70710678118654752f)) + hg[e] * 0.39894228040143268f * __expf(-0.5f * hg[e] * hg[e]);
   }
   if (MODE == FFN_UP_GELU) {
     if (a.h != nullptr) ffn_store8(a.h + row * a.N + f, x);
@@ -545,6 +552,12 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
       }
       for (int c = group * 32; MODE != FFN_DWEIGHT && c < t.n; c += 64) {
         uint32_t v[32];
+        FfnH h[4];
+        if (MODE == FFN_DACT_SWIGLU || MODE == FFN_DACT_GELU) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i * 8 + tr < t.n && f < a.N) ffn_load_h<MODE>(a, t.n0 + c + i * 8 + tr, f, h[i]);
+        }
         tmem_ld_32x32(t0 + c, v);
         tmem_ld_wait();
         ffn_turn_in(stg, v, lane);
@@ -589,7 +602,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
             if (c + j < t.n && f < a.N) {
               float x[8];
               ffn_turn_out(stg, j, part, x);
-              ffn_finish8<MODE>(a, t.n0 + c + j, f, x);
+              ffn_finish8<MODE>(a, t.n0 + c + j, f, x, h[i]);
             }
           }
           __syncwarp();
