@@ -82,17 +82,23 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(device, **tensors):
-    for name, t in tensors.items():
+def _on(device, *tensors):
+    for t in tensors:
         if t is not None and t.device != device:
-            _refuse(f"{name} is on {t.device}, not on {device}")
+            _refuse(f"a tensor is on {t.device}, not on {device} as the first one")
+
+
+def _first_derivative(backward):
+    """once_differentiable, whose own cost (4 us) is paid only where a graph of the gradients is wanted"""
+    slow = once_differentiable(backward)
+    return staticmethod(lambda ctx, *grads: slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads))
 
 
 # ------------------------------------------------------------------------------------------------ gate
 def _gate(logits, k, score, renormalize, bias, scale):
     T, G = logits.shape
-    ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
     weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+    ids = torch.empty_like(weights, dtype=torch.int32)
     _call("zepp_op_gate", logits.device, logits.data_ptr(), _TYPES[logits.dtype], T, G, k, score, renormalize, _ptr(bias),
           scale, ids.data_ptr(), weights.data_ptr())
     return ids, weights
@@ -108,8 +114,7 @@ class _Gate(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return ids, weights
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, _, dweights):
         if dweights is None:
             return (None,) * 6
@@ -141,7 +146,7 @@ def route_topk(logits, k, score="softmax", renormalize=True, bias=None, scale=1.
     if bias is not None:
         if score != "sigmoid" or bias.shape != (G,) or bias.dtype != torch.float32:
             _refuse("bias: float32 [experts], with sigmoid scores")
-        _on(logits.device, bias=bias)
+        _on(logits.device, bias)
         bias = bias.detach().contiguous()
     logits = logits.contiguous()
     args = (logits, int(k), _SCORES[score], int(bool(renormalize)), bias, float(scale))
@@ -159,11 +164,11 @@ class SortPlan(NamedTuple):
 def _sort(x, ids, num_experts, group_of):
     T, K = ids.shape
     H = x.shape[1]
-    rows = torch.empty((T * K, H), dtype=x.dtype, device=x.device)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=x.device)
-    position = torch.empty((T, K), dtype=torch.int32, device=x.device)
+    rows = x.new_empty((T * K, H))
+    offsets = ids.new_empty(num_experts + 1)
+    position = torch.empty_like(ids)
     ints = _fn("zepp_op_sort_ws_ints")(T, K, num_experts)
-    ws = torch.empty(ints, dtype=torch.int32, device=x.device) if ints else None
+    ws = ids.new_empty(ints) if ints else None
     _call("zepp_op_sort", x.device, x.data_ptr(), _TYPES[x.dtype], T, K, H, ids.data_ptr(), _ptr(group_of),
           0 if group_of is None else group_of.shape[0], num_experts, _ptr(ws), rows.data_ptr(), offsets.data_ptr(),
           position.data_ptr())
@@ -173,7 +178,7 @@ def _sort(x, ids, num_experts, group_of):
 def _unsort(rows, position, weights):
     T, K = position.shape
     H = rows.shape[1]
-    y = torch.empty((T, H), dtype=rows.dtype, device=rows.device)
+    y = rows.new_empty((T, H))
     _call("zepp_op_unsort", rows.device, rows.data_ptr(), _TYPES[rows.dtype], T, K, H, position.data_ptr(), _ptr(weights), y.data_ptr())
     return y
 
@@ -187,8 +192,7 @@ class _Sort(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return rows, offsets, position
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, drows, _offsets, _position):
         if drows is None:
             return None, None, None, None
@@ -203,15 +207,14 @@ class _Unsort(torch.autograd.Function):
         ctx.like = (rows.shape, rows.dtype)
         return _unsort(rows, position, weights)
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         rows, offsets, position, weights = ctx.saved_tensors
         dy = dy.contiguous()
         T, K = position.shape
         shape, dtype = ctx.like
-        drows = torch.empty(shape, dtype=dtype, device=dy.device) if ctx.needs_input_grad[0] else None
-        dweights = torch.empty((T, K), dtype=torch.float32, device=dy.device) if ctx.needs_input_grad[3] else None
+        drows = dy.new_empty(shape) if ctx.needs_input_grad[0] else None
+        dweights = torch.empty_like(weights) if ctx.needs_input_grad[3] else None
         _call("zepp_op_unsort_grad", dy.device, dy.data_ptr(), _ptr(rows), _TYPES[dtype], T, K, shape[1], offsets.shape[0] - 1,
               offsets.data_ptr(), position.data_ptr(), _ptr(weights), _ptr(drows), _ptr(dweights))
         return drows, None, None, dweights
@@ -233,7 +236,7 @@ def sort_tokens(x, ids, num_experts, group_of=None):
         if group_of.dim() != 1 or group_of.dtype != torch.int32:
             _refuse("group_of: a table of int32")
         group_of = group_of.contiguous()
-    _on(x.device, ids=ids, group_of=group_of)
+    _on(x.device, ids, group_of)
     args = (x.contiguous(), ids.contiguous(), int(num_experts), group_of)
     rows, offsets, position = _Sort.apply(*args) if x.requires_grad and torch.is_grad_enabled() else _sort(*args)
     return rows, SortPlan(offsets, position)
@@ -252,7 +255,7 @@ def unsort_tokens(rows, plan, weights=None):
         if weights.shape != (T, K) or weights.dtype != torch.float32:
             _refuse(f"weights: float32 [{T}, {K}], got {tuple(weights.shape)} {weights.dtype}")
         weights = weights.contiguous()
-    _on(rows.device, position=plan.position, offsets=plan.offsets, weights=weights)
+    _on(rows.device, plan.position, plan.offsets, weights)
     rows = rows.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _Unsort.apply(rows, plan.offsets.contiguous(), plan.position.contiguous(), weights)
@@ -270,7 +273,7 @@ def _ffn(rows, offsets, w1, w2, act, keep):
     G, f1 = w1.shape[:2]
     I = w2.shape[2]
     y = torch.empty_like(rows)
-    a = torch.empty((n, I), dtype=torch.bfloat16, device=rows.device)
+    a = rows.new_empty((n, I))
     h = torch.empty((n, f1), dtype=torch.float32, device=rows.device) if keep else None
     _call("zepp_op_expert_ffn", rows.device, rows.data_ptr(), n, offsets.data_ptr(), G, H, I, act, w1.data_ptr(), w2.data_ptr(),
           a.data_ptr(), _ptr(h), y.data_ptr())
@@ -285,8 +288,7 @@ class _ExpertFFN(torch.autograd.Function):
         ctx.act = act
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         rows, offsets, w1, w2, a, h = ctx.saved_tensors
         n, H = rows.shape
@@ -296,7 +298,7 @@ class _ExpertFFN(torch.autograd.Function):
         drows = torch.empty_like(rows) if need[0] else None
         dw1 = torch.empty_like(w1) if need[2] else None
         dw2 = torch.empty_like(w2) if need[3] else None
-        dh = torch.empty((n, f1), dtype=torch.bfloat16, device=rows.device) if need[0] or need[2] else None
+        dh = rows.new_empty((n, f1)) if need[0] or need[2] else None
         _call("zepp_op_expert_ffn_grad", rows.device, dy.data_ptr(), rows.data_ptr(), n, offsets.data_ptr(), G, H, w2.shape[2],
               ctx.act, w1.data_ptr(), w2.data_ptr(), a.data_ptr(), h.data_ptr(), _ptr(dh), _ptr(drows), _ptr(dw1), _ptr(dw2))
         return drows, None, dw1, dw2, None
@@ -320,7 +322,7 @@ def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
         _refuse("rows and weights are bfloat16, offsets int32")
     if H % 8 or I % 8 or H < 8 or I < 8 or not 1 <= G <= MAX_FFN_EXPERTS:
         _refuse(f"hidden and ffn are multiples of 8, 1..{MAX_FFN_EXPERTS} experts, got {H}, {I}, {G}")
-    _on(rows.device, offsets=offsets, w1=w1, w2=w2)
+    _on(rows.device, offsets, w1, w2)
     args = (_dense16(rows), offsets.contiguous(), _dense16(w1), _dense16(w2), _ACTS[act])
     if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
         return _ExpertFFN.apply(*args)
@@ -343,15 +345,19 @@ def _norm(tensors, max_norm):
     if not tensors:
         _refuse("no tensors")
     device = tensors[0].device
-    types = [_TYPES.get(t.dtype, 255) for t in tensors]
-    if device.type != "cuda" or max(types) > 2 or set(map(torch.Tensor.get_device, tensors)) != {device.index}:
+    dtypes = [t.dtype for t in tensors]
+    kinds = set(dtypes)
+    if device.type != "cuda" or not _TYPES.keys() >= kinds or set(map(torch.Tensor.get_device, tensors)) != {device.index}:
         _refuse("CUDA tensors of one device, of float32, bfloat16 or float16")
     if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.is_contiguous() or _is_dense(t) for t in tensors):
         _refuse("tensors whose elements lie without gaps and only once in memory")
     n = len(tensors)
     ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.uint64, n)
     sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
-    types = np.array(types, np.uint8)
+    if len(kinds) == 1:
+        types = np.full(n, _TYPES[dtypes[0]], np.uint8)
+    else:
+        types = np.fromiter(map(_TYPES.__getitem__, dtypes), np.uint8, n)
     if max_norm >= 0:
         some = sizes > 0
         first = ptrs[some]
