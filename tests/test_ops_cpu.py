@@ -56,8 +56,19 @@ def test_c_entry_points_refuse_before_any_gpu_call():
     assert "16-byte" in _error(ffn(8, 4, None, 2, 16, 8, 1, None, None, None, None, None, None))
     one, three = (ctypes.c_int64 * 1)(4), bytes([3])
     norm = f("zepp_op_grad_norm")
-    assert "element type" in _error(norm((ctypes.c_void_p * 1)(16), one, three, 1, 1.0, None, None, None))
-    assert "aligned" in _error(norm((ctypes.c_void_p * 1)(2), one, bytes([0]), 1, 1.0, None, None, None))
+    assert "element type" in _error(norm((ctypes.c_void_p * 1)(16), one, three, 1, 1.0, 16, 16, None))
+    assert "aligned" in _error(norm((ctypes.c_void_p * 1)(2), one, bytes([0]), 1, 1.0, 16, 16, None))
+    # what a call cannot do without
+    for rc in (f("zepp_op_gate")(None, 0, 1, 8, 2, 0, 1, None, 1.0, 16, 16, None),
+               f("zepp_op_gate_grad")(16, 0, 1, 8, 2, 0, 1, 1.0, 16, 16, None, 16, None),
+               f("zepp_op_sort")(16, 0, 1, 2, 8, None, None, 0, 8, None, 16, 16, 16, None),
+               f("zepp_op_unsort")(16, 0, 1, 2, 8, None, None, 16, None),
+               f("zepp_op_unsort_grad")(None, 16, 0, 1, 2, 8, 4, 16, 16, None, 16, None, None),
+               ffn(16, 4, None, 2, 16, 8, 1, 16, 16, 16, None, 16, None),
+               f("zepp_op_expert_ffn_grad")(16, 16, 4, 16, 2, 16, 8, 1, 16, 16, 16, 16, None, 16, None, None, None),
+               norm((ctypes.c_void_p * 1)(0), one, bytes([0]), 1, 1.0, 16, 16, None), norm(None, None, None, 1, 1.0, 16, 16, None),
+               norm(None, None, None, 0, 1.0, None, 16, None)):
+        assert "null pointer" in _error(rc)
 
 
 def test_sizes():

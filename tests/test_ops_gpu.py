@@ -290,7 +290,10 @@ def near(got, want, what):
 FFN_CASES = [
     ((1,), 8, 8, "swiglu", 0), ((0, 3, 0), 64, 64, "swiglu", 2), ((130, 0, 1, 64, 65, 127), 136, 72, "swiglu", 3),
     ((33, 16, 15, 17, 0, 48), 392, 136, "gelu", 5), ((300,), 256, 384, "swiglu", 0), ((129, 256, 40), 520, 264, "gelu", 0),
-    ((0, 0), 128, 128, "swiglu", 4), (tuple(range(40)), 192, 128, "swiglu", 1), ((5,) * 128, 256, 128, "gelu", 0)]
+    ((0, 0), 128, 128, "swiglu", 4), (tuple(range(40)), 192, 128, "swiglu", 1), ((5,) * 128, 256, 128, "gelu", 0),
+    ((500, 40, 0, 390), 520, 264, "swiglu", 0), ((3,) * 400, 136, 72, "swiglu", 1), ((2,) * 1024, 64, 64, "gelu", 0),
+    # several column tiles of a weight gradient in a row, for experts short and long
+    ((0, 1, 15, 16, 17, 63, 64, 65, 0, 383, 384, 385, 700) + tuple((7 * i) % 97 for i in range(115)), 1024, 512, "swiglu", 9)]
 
 
 @pytest.mark.parametrize("counts, H, I, act, spare", FFN_CASES)
@@ -718,3 +721,49 @@ def test_unsort_of_many_long_rows(T, K, H, dtype):
     assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r, plan, w.detach()), r, dy)[0], dr)       # without dweights
     assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r.detach(), plan, w), w, dy)[0], dw)       # without drows
     ops.check_waits()
+
+
+def test_expert_ffn_without_rows():
+    w1, w2 = randn((3, 32, 24), gen(1), torch.bfloat16), randn((3, 24, 16), gen(1), torch.bfloat16)
+    leaves = [torch.zeros((0, 24), dtype=torch.bfloat16, device="cuda"), w1, w2]
+    for t in leaves:
+        t.requires_grad_(True)
+    y = zb.expert_ffn(leaves[0], torch.zeros(4, dtype=torch.int32, device="cuda"), w1, w2)
+    assert y.shape == (0, 24)
+    dx, d1, d2 = torch.autograd.grad(y, leaves, torch.zeros_like(y))
+    assert dx.shape == (0, 24) and d1.shape == w1.shape and not d1.any() and not d2.any()
+
+
+def test_gradients_are_first_derivatives_only():
+    """With create_graph the gradients come out the same; a second derivative is an error, not a wrong number."""
+    l = randn((5, 16), gen(2)).requires_grad_(True)
+    w = zb.route_topk(l, 3)[1]
+    once = torch.autograd.grad(w.square().sum(), l, retain_graph=True)[0]
+    twice = torch.autograd.grad(w.square().sum(), l, create_graph=True)[0]
+    assert torch.equal(once, twice)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(twice.sum(), l)
+
+
+def test_padded_batch_through_the_whole_chain():
+    """Pad rows (logits masked out) cost nothing and change nothing: the real tokens' results are those of the batch without
+    them, and pad tokens get zeros, in both directions."""
+    T, pads, G, H, I, K = 70, 26, 12, 128, 72, 3
+    g = gen(31)
+    logits, x = randn((T, G), g), randn((T, H), g, torch.bfloat16)
+    w1, w2 = randn((G, 2 * I, H), g, torch.bfloat16, 0.1), randn((G, H, I), g, torch.bfloat16, 0.1)
+    dy = randn((T, H), g, torch.bfloat16)
+    res = []
+    for n in (0, pads):
+        l = torch.cat([logits, torch.full((n, G), -math.inf, device="cuda")]).requires_grad_(True)
+        xs = torch.cat([x, torch.full((n, H), math.nan, dtype=torch.bfloat16, device="cuda")]).requires_grad_(True)
+        a, b = w1.clone().requires_grad_(True), w2.clone().requires_grad_(True)
+        ids, w = zb.route_topk(l, K, renormalize=False)
+        rows, plan = zb.sort_tokens(xs, ids, G)
+        y = zb.unsort_tokens(zb.expert_ffn(rows, plan.offsets, a, b), plan, w)
+        d = torch.cat([dy, torch.full((n, H), math.nan, dtype=torch.bfloat16, device="cuda")])
+        gl, gx, ga, gb = torch.autograd.grad(y, (l, xs, a, b), d)
+        assert not y[T:].any() and not gl[T:].any() and not gx[T:].any()
+        res.append((y[:T], gl[:T], gx[:T], ga, gb))
+    for u, v in zip(*res):
+        assert torch.equal(u, v)

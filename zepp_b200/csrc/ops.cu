@@ -2,6 +2,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/zepp_b200.h"
@@ -88,6 +89,12 @@ int op_device(OpDevice** out) {
 }
 
 int elem_bytes(int dtype) { return dtype == OP_F32 ? 4 : 2; }
+// none of the pointers that a call cannot do without is null
+bool given(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (p == nullptr) return false;
+  return true;
+}
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 }  // namespace
@@ -147,6 +154,7 @@ extern "C" int zepp_op_gate(const void* logits, int dtype, int64_t T, int G, int
                             const float* bias, float scale, int32_t* ids, float* weights, void* stream) {
   if (int rc = gate_check("gate", dtype, T, G, k, sigmoid)) return rc;
   if (bias != nullptr && !sigmoid) return fail("gate: a balancing bias goes with sigmoid scores");
+  if (T > 0 && !given({logits, ids, weights})) return fail("gate: null pointer");
   GateArgs a{};
   a.logits = logits; a.T = T; a.G = G; a.k = k; a.sigmoid = sigmoid; a.renormalize = renormalize; a.bias = bias; a.scale = scale;
   a.ids = ids; a.weights = weights;
@@ -157,6 +165,7 @@ extern "C" int zepp_op_gate_grad(const void* logits, int dtype, int64_t T, int G
                                  float scale, const int32_t* ids, const float* weights, const float* dweights,
                                  void* dlogits, void* stream) {
   if (int rc = gate_check("gate_grad", dtype, T, G, k, sigmoid)) return rc;
+  if (T > 0 && !given({logits, ids, weights, dweights, dlogits})) return fail("gate_grad: null pointer");
   GateArgs a{};
   a.logits = logits; a.T = T; a.G = G; a.k = k; a.sigmoid = sigmoid; a.renormalize = renormalize; a.scale = scale;
   a.ids = const_cast<int32_t*>(ids); a.weights = const_cast<float*>(weights);
@@ -185,6 +194,7 @@ extern "C" int zepp_op_sort(const void* x, int dtype, int64_t T, int K, int64_t 
                             int32_t* position, void* stream) {
   if (int rc = sort_check("sort", dtype, T, K, H)) return rc;
   if (G < 1 || G > kSortMaxGroups) return fail("sort: 1..%d experts (got %d)", kSortMaxGroups, G);
+  if (offsets == nullptr || (T > 0 && !given({x, ids, rows, position}))) return fail("sort: null pointer");
   OpDevice* d;
   if (int rc = op_device(&d)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -274,6 +284,7 @@ extern "C" int zepp_op_unsort(const void* rows, int dtype, int64_t T, int K, int
                               const float* weights, void* y, void* stream) {
   if (int rc = sort_check("unsort", dtype, T, K, H)) return rc;
   if (T == 0) return 0;
+  if (!given({rows, position, y})) return fail("unsort: null pointer");
   UnsortArgs a{};
   a.rows = rows; a.T = T; a.N = T * K; a.K = K; a.H = H; a.position = position; a.weights = weights; a.y = y;
   return unsort_run(a, dtype, false, stream);
@@ -285,6 +296,7 @@ extern "C" int zepp_op_unsort_grad(const void* dy, const void* rows, int dtype, 
   if (int rc = sort_check("unsort_grad", dtype, T, K, H)) return rc;
   if (G < 1) return fail("unsort_grad: no experts");
   if (T == 0 || (drows == nullptr && dweights == nullptr)) return 0;
+  if (!given({dy, offsets, position})) return fail("unsort_grad: null pointer");
   if (dweights != nullptr && rows == nullptr) return fail("unsort_grad: the weights' gradient needs the rows");
   UnsortArgs a{};
   a.dy = dy; a.rows = rows; a.T = T; a.N = T * K; a.K = K; a.H = H; a.position = position; a.weights = weights;
@@ -382,6 +394,7 @@ extern "C" int zepp_op_expert_ffn(const void* rows, int64_t n, const int32_t* of
                                   const void* w1, const void* w2, void* a_out, void* h_out, void* y, void* stream) {
   if (int rc = ffn_check("expert_ffn", n, G, H, I, act, {rows, w1, w2, a_out, h_out, y})) return rc;
   if (n == 0) return 0;
+  if (!given({rows, offsets, w1, w2, a_out, y})) return fail("expert_ffn: null pointer");
   FfnCall c{offsets, n, G, H, I, act, nullptr, static_cast<cudaStream_t>(stream)};
   if (int rc = op_device(&c.dev)) return rc;
   if (act) {
@@ -403,6 +416,8 @@ extern "C" int zepp_op_expert_ffn_grad(const void* dy, const void* rows, int64_t
     if (dw2 != nullptr) CU_OK(cudaMemsetAsync(dw2, 0, (size_t)G * H * I * 2, s));
     return 0;
   }
+  if (!given({dy, rows, offsets, w1, w2, a, h}) || ((drows != nullptr || dw1 != nullptr) && dh_ws == nullptr))
+    return fail("expert_ffn_grad: null pointer");
   if (int rc = op_device(&c.dev)) return rc;
   if (drows != nullptr || dw1 != nullptr) {
     if (act) {
@@ -489,9 +504,11 @@ static int norm_run(void* const* ptrs, const int64_t* sizes, const uint8_t* dtyp
 extern "C" int zepp_op_grad_norm(void* const* ptrs, const int64_t* sizes, const uint8_t* dtypes, int count, double max_norm,
                                  float* norm, void* ws, void* stream) {
   if (count < 0) return fail("grad_norm: %d tensors", count);
+  if (!given({norm, ws}) || (count > 0 && !given({ptrs, sizes, dtypes}))) return fail("grad_norm: null pointer");
   for (int i = 0; i < count; ++i) {
     if (dtypes[i] > OP_F16) return fail("grad_norm: unknown element type %d of tensor %d", dtypes[i], i);
     if (sizes[i] < 0 || sizes[i] >= (1ll << 45)) return fail("grad_norm: %lld elements in tensor %d", (long long)sizes[i], i);
+    if (sizes[i] > 0 && ptrs[i] == nullptr) return fail("grad_norm: tensor %d is a null pointer", i);
     if (sizes[i] > 0 && !aligned(ptrs[i], elem_bytes(dtypes[i]))) return fail("grad_norm: tensor %d is not aligned to its elements", i);
   }
   OpDevice* d;

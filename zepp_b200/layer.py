@@ -314,6 +314,8 @@ class EPMoE(torch.nn.Module):
             dem = self._h.table("demands").cpu().tolist()
             d = Demands(*[int(v) for v in dem[:7]])
             raise CapacityExceeded(violations(d, self.caps, direct=self.cfg.comm_strategy == "direct"), d)
+        if self._group_of is not None:        # forward_train ran: its operators' waits too
+            ops.check_waits(self.device)
         if st[0]:
             what = ", ".join(n for b, n in _ERR_NAMES.items() if st[0] & b)
             raise RuntimeError(f"zepp_b200 step failed: {what} (wait id {st[1]}, peer/item {st[2]}, epoch {st[3]})")
