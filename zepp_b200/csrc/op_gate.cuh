@@ -12,7 +12,7 @@
 // register j, four neighbours per access.  The (k + 1)-th largest of the 32 lanes' largest keys (order-preserving
 // integers, redux.sync) is a bound that hardly more than k keys reach; those few are put together, one per lane, and each
 // counts the ones before it (up to k = 20 or so they are fewer than 32; a row with more goes through 64 bits).  That is about 20 instructions per place, where k rounds of a maximum over all registers took
-// 200 (16381 rows of 384 bf16 logits with a bias: 30 us against 45 us).  Bound by instruction issue.
+// 200 (16381 rows of 384 bf16 logits with a bias: 25 us against 45 us).  Bound by instruction issue.
 #pragma once
 #include "op_common.cuh"
 
@@ -75,8 +75,10 @@ __device__ __forceinline__ void gate_load(const T* row, int G, int lane, bool ve
 
 __device__ __forceinline__ float sigmoid_f32(float l) { return 1.0f / (1.0f + expf(-l)); }
 
-// The choice by the scores in 64 bits, straight from the row: for rows where the balanced scores of two neighbours of the
-// order lie within the rounding of the 32-bit values, and for rows with too many equal values to sort them in one warp.
+// 1 / (1 + exp(-l)) + bias in 64 bits
+__device__ __noinline__ double gate_score_f64(float l, float bias) { return 1.0 / (1.0 + exp(-(double)l)) + (double)bias; }
+
+// The choice by the scores in 64 bits, straight from the row: for rows with too many equal values to sort them in one warp.
 // Lane j < k returns its choice, -1 where none is left.
 template <typename T, int NPL>
 __device__ __noinline__ int gate_choose_f64(const T* row, const float* bias, int G, int k, int lane) {
@@ -88,7 +90,7 @@ __device__ __noinline__ int gate_choose_f64(const T* row, const float* bias, int
     if (i < G) {
       const float l = to_f32<T>(row[i]);
       if (l > -INFINITY) {
-        const double v = bias != nullptr ? 1.0 / (1.0 + exp(-(double)l)) + (double)bias[i] : (double)l;
+        const double v = bias != nullptr ? gate_score_f64(l, bias[i]) : (double)l;
         if (v > -INFINITY) key[j] = v;                 // false for NaN
       }
     }
@@ -152,6 +154,14 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a)
     bound = __reduce_max_sync(0xffffffffu, best);
   }
   if (bound == 0) bound = 1;                         // fewer lanes than that: every key that can be chosen
+  // A 32-bit score is off by at most 1.6e-6 s (1 - s) <= 4e-7 for the exponential (its argument is rounded, |l| <= 16 where
+  // s (1 - s) matters), 1.2e-7 for the quotient and half a step of s + bias: two of them may be in the wrong order where
+  // they are less than `slack` apart.  What is that little below the bound is a candidate too.
+  auto slack = [](float v) { return 2e-6f + 2.4e-7f * fabsf(v); };
+  if (a.bias != nullptr && bound > 1) {
+    const float v = gate_value(bound);
+    bound = max(gate_key(v - slack(v)), 1u);
+  }
   int cnt = 0;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) cnt += key[j] >= bound ? 1 : 0;
@@ -183,11 +193,23 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a)
     const uint2 chosen = s_order[warp][lane < a.k ? lane : a.k];
     if (lane < a.k) mine = (int)chosen.y;
     if (a.bias != nullptr) {
-      // A 32-bit score is off by at most 1.6e-6 s (1 - s) <= 4e-7 for the exponential (its argument is rounded, |l| <= 16
-      // where s (1 - s) matters), 1.2e-7 for the quotient and half a step of s + bias; twice that for two of them.
       const uint2 next = s_order[warp][lane < a.k ? lane + 1 : a.k];
-      const float v = gate_value(chosen.x), w = gate_value(next.x);
-      again = __any_sync(0xffffffffu, lane < a.k && next.x != 0u && v - w <= 2e-6f + 2.4e-7f * fabsf(v));
+      const float v = gate_value(chosen.x);
+      if (__any_sync(0xffffffffu, lane < a.k && next.x != 0u && v - gate_value(next.x) <= slack(v))) {
+        // in doubt: the candidates once more, by their scores in 64 bits
+        const bool real = lane < n;
+        const double score = real ? gate_score_f64(to_f32<T>(src[me.y]), a.bias[me.y]) : 0.0;
+        rank = 0;
+        for (int c = 0; c < n; ++c) {
+          const double o = __shfl_sync(0xffffffffu, score, c);
+          const unsigned i = __shfl_sync(0xffffffffu, me.y, c);
+          rank += o > score || (o == score && i < me.y) ? 1 : 0;
+        }
+        __syncwarp();
+        if (real && rank < a.k) s_order[warp][rank] = me;
+        __syncwarp();
+        if (lane < a.k) mine = (int)s_order[warp][lane].y;
+      }
     }
   }
   if (again) mine = gate_choose_f64<T, NPL>(src, a.bias, a.G, a.k, lane);
