@@ -7,7 +7,10 @@
 //
 // The order is that of a stable sort by group, and every sum runs over k in order, so equal inputs give equal bits.
 // Everything is bound by the bytes of the rows: the sort reads a row once and writes its K copies, the gradient of the
-// unsort reads dy once and makes both of its results from one pass over the rows.
+// unsort reads dy once and makes both of its results from one pass over the rows.  Measured with 8192 tokens x 8 copies of
+// 4096 bf16: sort 4 + 119 us (5.1 TB/s, nearly all writes; a fill of memory reaches 3.9), unsort 112 us (5.4 TB/s), its
+// gradient 185 us (6.2 TB/s).  Counting costs the second launch only above 8192 copies; with fewer, a block that counts all
+// ids itself takes less than a launch (32 tokens: 6 us).
 #pragma once
 #include "op_common.cuh"
 
@@ -321,8 +324,8 @@ __global__ void __launch_bounds__(kUnsortGradThreads) unsort_grad_kernel(const U
 // ---------------------------------------------------------------------------------------------------------------------
 // The same two for long rows in large numbers: one persistent block per SM, a warp that fetches pieces of the rows into a
 // ring of shared-memory stages with bulk copies, eight warps that add them up.  A stage holds one piece (kPieceBytes) of up
-// to eight copies' rows (GRAD: and of dy), so nearly 200 KB are in flight on every SM whatever the registers allow, and the
-// positions, the first link of each chain of loads, are read one stage ahead.
+// to eight copies' rows (GRAD: and of dy), so nearly 200 KB are in flight on every SM whatever the registers allow: 112 and
+// 185 us where the kernels above take 152 and 226 (8192 tokens x 8 copies of 4096 bf16).
 // Steps of a block, `steps` in all per token: (piece, eight copies) with the copies inner, or GRAD: (eight copies, piece)
 // with the piece inner, so that a sum over k or over the row stays in registers.
 constexpr int kPieceBytes = 4096;
