@@ -767,3 +767,35 @@ def test_padded_batch_through_the_whole_chain():
         res.append((y[:T], gl[:T], gx[:T], ga, gb))
     for u, v in zip(*res):
         assert torch.equal(u, v)
+
+
+def test_calls_of_every_kind_of_argument():
+    """Gradients through what is optional or copied on the way: no weights, transposed weights, generators, views."""
+    g = gen(41)
+    ids = torch.randint(-1, 5, (30, 3), generator=g, device="cuda", dtype=torch.int32)
+    _, plan = zb.sort_tokens(randn((30, 16), g), ids, 5)
+    r = randn((90, 16), g).requires_grad_(True)
+    dy = randn((30, 16), g)
+    dr = torch.autograd.grad(zb.unsort_tokens(r, plan), r, dy)[0]
+    want = torch.zeros(90, 16, device="cuda")
+    t, k = (plan.position >= 0).nonzero(as_tuple=True)
+    want[plan.position[t, k].long()] = dy[t]
+    assert torch.equal(dr, want)
+    # weights held the other way round: the gradient comes back in their layout
+    x, offsets, w1, w2, d, _ = ffn_inputs((20, 30), 64, 40, "swiglu", 0, 42)
+    flip = w1.transpose(1, 2).contiguous().requires_grad_(True)
+    plain = w1.clone().requires_grad_(True)
+    a = torch.autograd.grad(zb.expert_ffn(x, offsets, flip.transpose(1, 2), w2), flip, d)[0]
+    b = torch.autograd.grad(zb.expert_ffn(x, offsets, plain, w2), plain, d)[0]
+    assert torch.equal(a, b.transpose(1, 2))
+    # a part of a longer buffer, and every other offset of a table
+    wide = torch.stack([offsets, offsets], 1)
+    assert torch.equal(zb.expert_ffn(torch.cat([x, x])[:50], wide[:, 0], w1, w2), zb.expert_ffn(x, offsets, w1, w2))
+    ts = [randn((7,), g), randn((), g)]
+    before = [t.clone() for t in ts]
+    n = zb.clip_grad_norm_((t for t in ts), math.inf)
+    assert all(torch.equal(u, v) for u, v in zip(ts, before)) and float(n) > 0
+    with torch.inference_mode():
+        w = zb.route_topk(randn((4, 8), g), 2)[1]
+        assert torch.allclose(w.sum(1), torch.ones(4, device="cuda"), atol=1e-6)
+        zb.clip_grad_norm_([torch.ones(4, device="cuda")], 1.0)
