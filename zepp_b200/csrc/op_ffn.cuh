@@ -77,6 +77,12 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// Arrival on a barrier of either CTA that says no more than that this thread's TMEM reads are done (tcgen05.fence before it).
+// A release at cluster scope would also wait for the thread's stores to global memory: 3600 cycles per tile of a weight
+// gradient, more than half of the epilogue.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
+}
 // Once a wait for this phase has returned: what the other CTA of the cluster did before its arrival is visible too.
 __device__ __forceinline__ void mbar_acquire_cluster(uint64_t* bar, uint32_t parity) {
   asm volatile(
@@ -615,7 +621,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
       if (left) break;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(lead_acc_empty + 8u * (uint32_t)acc);
+      if (lane == 0) mbar_arrive_pair(lead_acc_empty + 8u * (uint32_t)acc);
       if (++acc == kAccStages) { acc = 0; acc_phase ^= 1; }
     }
   }
