@@ -77,19 +77,14 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// Arrival on a barrier of either CTA that says no more than that this thread's TMEM reads are done (tcgen05.fence before it).
-// A release at cluster scope would also wait for the thread's stores to global memory: 3600 cycles per tile of a weight
-// gradient, more than half of the epilogue.
+// Arrival on a barrier of either CTA.  What it announces is ordered by a fence of its own before it: TMEM reads by
+// tcgen05.fence, shared memory that an MMA will read by fence.proxy.async.  A release at cluster scope would wait for more,
+// the thread's stores to global memory among it: 3600 cycles for the epilogue of a weight gradient's tile, 3300 for clearing rows.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
 }
-// Once a wait for this phase has returned: what the other CTA of the cluster did before its arrival is visible too.
-__device__ __forceinline__ void mbar_acquire_cluster(uint64_t* bar, uint32_t parity) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}"
-      ::"r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+__device__ __forceinline__ void fence_proxy_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 // One lane of a converged warp, always the same.  The copies and MMAs take their operands from uniform registers: issued
 // under `lane == 0` they cost 570 cycles per K step on the issuing thread (380 of them without a single MMA), more than
@@ -452,10 +447,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
             break;
           }
           int steps = 4;
-          if (MODE == FFN_DWEIGHT && kb == t.k_steps - 1) {
-            steps = (t.k_rows - kb * 64 + 15) / 16;
-            mbar_acquire_cluster(&full_bar[stage], phase);      // the rows that the other CTA cleared
-          }
+          if (MODE == FFN_DWEIGHT && kb == t.k_steps - 1) steps = (t.k_rows - kb * 64 + 15) / 16;
           tc_fence_after();
           const uint32_t sf = smem_u32(smem + (size_t)stage * kFfnStageBytes), sr = sf + kFfnHalfBytes;
           const uint64_t fd = kWeightsK ? make_kmajor_sw128_desc(sf) : make_mnmajor_sw128_desc(sf);
@@ -504,9 +496,9 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
           uint8_t* at = smem + (size_t)stage * kFfnStageBytes + (lane >> 3) * kFfnBlockBytes + (lane & 7) * 16;
           const int used = (t.k_rows - 1) % 64 + 1;
           for (int r = used; r < used + foreign; ++r) *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async();
+          fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(lead_full + 8u * (uint32_t)stage);
+          if (lane == 0) mbar_arrive_pair(lead_full + 8u * (uint32_t)stage);
         }
         if (++stage == stages) stage = 0;
       }
