@@ -490,6 +490,26 @@ def test_clip_orders_gaps_overlaps():
 
 
 # ------------------------------------------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("n", (2, 16, 17, 40))
+def test_clip_neighbours_and_overlaps_by_count(n):
+    """Short and long lists: tensors that touch are taken in any order, one shared element is refused."""
+    buf = torch.ones(n * 64, device="cuda")
+    parts = [buf[i * 64:(i + 1) * 64] for i in range(n)][::-1]
+    parts[0] = parts[0].to(torch.bfloat16)
+    parts += [buf[64:64]]                                                    # empty, inside another's span
+    total = zb.clip_grad_norm_(parts, 1.0)
+    # all summands are 1: sums of integers below 2^24 are exact, one rounding of the root and the type's own
+    assert abs(float(total) - math.sqrt(n * 64)) <= 2 * U * math.sqrt(n * 64)
+    kept = buf.clone()
+    more = [torch.ones(64, device="cuda") for _ in range(n - 2)] + [buf[:64], buf[63:100]]
+    with pytest.raises(AssertionError):
+        zb.clip_grad_norm_(more, 1.0)
+    assert torch.equal(buf, kept) and all(bool((t == 1).all()) for t in more[:-2])
+    want = math.sqrt(sum(float(t.double().square().sum()) for t in more))
+    # order of the kernel's sums is free: (64 n + 37) summands in fp32 at most lose one U each in the sum, half in the root
+    assert abs(float(zb.grad_norm(more)) - want) <= (64 * n + 40) * U * want
+
+
 def test_refusals():
     c = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
     i32, bf = dict(dtype=torch.int32), dict(dtype=torch.bfloat16)

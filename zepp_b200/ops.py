@@ -352,23 +352,34 @@ def _norm(tensors, max_norm):
     if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.is_contiguous() or _is_dense(t) for t in tensors):
         _refuse("tensors whose elements lie without gaps and only once in memory")
     n = len(tensors)
-    ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.uint64, n)
-    sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
-    if len(kinds) == 1:
-        types = np.full(n, _TYPES[dtypes[0]], np.uint8)
-    else:
-        types = np.fromiter(map(_TYPES.__getitem__, dtypes), np.uint8, n)
-    if max_norm >= 0:
-        some = sizes > 0
-        first = ptrs[some]
-        last = first + (sizes[some] * np.where(types[some] == 0, 4, 2)).astype(np.uint64)
-        order = first.argsort()
-        if (first[order[1:]] < last[order[:-1]]).any():
-            _refuse("tensors that do not overlap (one is given twice?)")
     out = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(_fn("zepp_op_grad_norm_ws_bytes")(n), dtype=torch.uint8, device=device)
-    _call("zepp_op_grad_norm", device, ptrs.ctypes.data, sizes.ctypes.data, types.ctypes.data, n, max_norm, out.data_ptr(),
-          ws.data_ptr())
+    # Short lists in plain Python, long ones in numpy, whose calls have a fixed cost. Host time of a clipping call, plain
+    # against numpy: 19 and 29 us for 1 tensor, 25 and 33 for 8, 30 and 36 for 16; of a norm alone 17 and 21, 21 and 23, 25 and 25.
+    if n <= 16:
+        ptrs, sizes, types = [t.data_ptr() for t in tensors], [t.numel() for t in tensors], [_TYPES[d] for d in dtypes]
+        if max_norm >= 0:
+            spans = sorted((p, p + c * (2 if ty else 4)) for p, c, ty in zip(ptrs, sizes, types) if c)
+            overlap = any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+        tables = (_P * n)(*ptrs), (_L * n)(*sizes), (ctypes.c_uint8 * n)(*types)
+        at = [ctypes.addressof(t) for t in tables]
+    else:
+        ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.uint64, n)
+        sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
+        if len(kinds) == 1:
+            types = np.full(n, _TYPES[dtypes[0]], np.uint8)
+        else:
+            types = np.fromiter(map(_TYPES.__getitem__, dtypes), np.uint8, n)
+        if max_norm >= 0:
+            some = sizes > 0
+            first = ptrs[some]
+            last = first + (sizes[some] * np.where(types[some] == 0, 4, 2)).astype(np.uint64)
+            order = first.argsort()
+            overlap = (first[order[1:]] < last[order[:-1]]).any()
+        at = [t.ctypes.data for t in (ptrs, sizes, types)]
+    if max_norm >= 0 and overlap:
+        _refuse("tensors that do not overlap (one is given twice?)")
+    _call("zepp_op_grad_norm", device, *at, n, max_norm, out.data_ptr(), ws.data_ptr())
     return out
 
 
