@@ -1,0 +1,46 @@
+"""The operators around the layer at their edges: what neighbours, special values, streams and failures may not change."""
+import math
+
+import pytest
+import torch
+
+import zepp_b200 as zb
+from zepp_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, g, dtype=torch.float32, std=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * std).to(dtype)
+
+
+# -------------------------------------------------------------------------------------------------- experts' products
+@pytest.mark.parametrize("act, experts, most, H, I", [("swiglu", 200, 150, 512, 256), ("gelu", 97, 400, 1032, 264), ("swiglu", 600, 31, 256, 128)])
+def test_expert_ffn_rows_of_neighbours_never_reach_a_weight_gradient(act, experts, most, H, I):
+    """The last step of an expert's sum holds rows of the next expert, which are cleared by both CTAs of a pair.  Over many
+    waves of tiles, with NaN and infinities in every second expert's rows, the experts between them get the same bits as
+    with clean neighbours, every time."""
+    g = gen(experts)
+    counts = torch.randint(0, most, (experts,), generator=g, device="cuda")
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).int()
+    n = int(offsets[-1])
+    f1 = I * (2 if act == "swiglu" else 1)
+    x, dy = randn((n, H), g, torch.bfloat16), randn((n, H), g, torch.bfloat16)
+    w1, w2 = randn((experts, f1, H), g, torch.bfloat16, H ** -0.5), randn((experts, H, I), g, torch.bfloat16, I ** -0.5)
+    expert = torch.repeat_interleave(torch.arange(experts, device="cuda"), counts)
+    odd = (expert % 2 == 1)[:, None]
+    res = []
+    for change in (lambda t, v: t, lambda t, v: torch.where(odd, torch.full_like(t, v), t)):
+        leaves = [change(x, math.nan).requires_grad_(True), w1.clone().requires_grad_(True), w2.clone().requires_grad_(True)]
+        y = zb.expert_ffn(leaves[0], offsets, leaves[1], leaves[2], act=act)
+        for _ in range(20 if res else 1):
+            _, d1, d2 = torch.autograd.grad(y, leaves, change(dy, math.inf), retain_graph=True)
+            res.append((d1[::2], d2[::2]))
+    assert bool(res[0][0].isfinite().all()) and bool(res[0][1].isfinite().all())
+    for a, b in res[1:]:
+        assert torch.equal(a, res[0][0]) and torch.equal(b, res[0][1])
+    ops.check_waits()

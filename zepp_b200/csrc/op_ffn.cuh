@@ -77,12 +77,30 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// Arrival on a barrier of either CTA.  What it announces is ordered by a fence of its own before it: TMEM reads by
-// tcgen05.fence, shared memory that an MMA will read by fence.proxy.async.  A release at cluster scope would wait for more,
-// the thread's stores to global memory among it: 3600 cycles for the epilogue of a weight gradient's tile, 3300 for clearing rows.
+// Arrival on a barrier of either CTA of the pair, at the scope of both (a CTA-scoped one does not order anything for a thread
+// of the other CTA).  Relaxed: what it announces is ordered by a fence of its own before it, TMEM reads by tcgen05.fence,
+// cleared rows by the two below.  With release semantics the arrival would also wait for the thread's stores to global
+// memory: 3600 cycles for the epilogue of a weight gradient's tile, 3300 for clearing rows.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_addr) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
 }
+// The other side, once a bounded wait for this phase has returned: the same phase seen at the pair's scope.
+__device__ __forceinline__ void mbar_seen_pair(uint64_t* bar, uint32_t parity) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 p, [%0], %1;\n\t}"
+      ::"r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+}
+// Stores to this CTA's shared memory, made before the arrival that follows, for the thread that waits for it in either CTA ...
+__device__ __forceinline__ void fence_release_pair_shared() {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+// ... and that thread's side of it
+__device__ __forceinline__ void fence_acquire_pair_shared() {
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+}
+// this thread's stores to shared memory before what the copies and MMAs do there
 __device__ __forceinline__ void fence_proxy_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -438,6 +456,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
           if (lane == 0) give_up(WAIT_TMEM_EMPTY, item, acc);
           break;
         }
+        mbar_seen_pair(&acc_empty_bar[acc], acc_phase ^ 1);
         tc_fence_after();
         const uint32_t d0 = tmem_base + acc * 256;
         for (int kb = 0; kb < t.k_steps; ++kb) {
@@ -447,7 +466,13 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
             break;
           }
           int steps = 4;
-          if (MODE == FFN_DWEIGHT && kb == t.k_steps - 1) steps = (t.k_rows - kb * 64 + 15) / 16;
+          if (MODE == FFN_DWEIGHT && kb == t.k_steps - 1) {
+            steps = (t.k_rows - kb * 64 + 15) / 16;
+            if (ffn_foreign(t.k_rows) != 0) {            // both CTAs' cleared rows
+              mbar_seen_pair(&full_bar[stage], phase);
+              fence_acquire_pair_shared();
+            }
+          }
           tc_fence_after();
           const uint32_t sf = smem_u32(smem + (size_t)stage * kFfnStageBytes), sr = sf + kFfnHalfBytes;
           const uint64_t fd = kWeightsK ? make_kmajor_sw128_desc(sf) : make_mnmajor_sw128_desc(sf);
@@ -498,7 +523,10 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
           for (int r = used; r < used + foreign; ++r) *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive_pair(lead_full + 8u * (uint32_t)stage);
+          if (lane == 0) {
+            fence_release_pair_shared();
+            mbar_arrive_pair(lead_full + 8u * (uint32_t)stage);
+          }
         }
         if (++stage == stages) stage = 0;
       }
