@@ -209,6 +209,10 @@ size_t zepp_op_grad_norm_ws_bytes(int count);
 int zepp_op_grad_norm(void* const* ptrs, const int64_t* sizes, const uint8_t* dtypes, int count, double max_norm,
                       float* norm_dev, void* ws_dev, void* stream);
 
+/* How long a bounded wait inside an operator's kernel lasts before the kernel gives up (its outputs are then incomplete and
+ * zepp_op_status says so); for the calls of this process from now on, 2 s where nothing was set. */
+int zepp_op_set_wait_limit_ns(int64_t ns);
+
 /* Deferred verdict of the operators' bounded waits on the current device: synchronises `stream`, copies 8 status words
  * (as zepp_layer_status) and clears them. */
 int zepp_op_status(void* stream, uint64_t out[8]);

@@ -44,3 +44,41 @@ def test_expert_ffn_rows_of_neighbours_never_reach_a_weight_gradient(act, expert
     for a, b in res[1:]:
         assert torch.equal(a, res[0][0]) and torch.equal(b, res[0][1])
     ops.check_waits()
+
+
+# ------------------------------------------------------------------------------------------------- waits that run out
+@pytest.fixture
+def no_patience():
+    ops.set_wait_limit(0)
+    yield
+    ops.set_wait_limit(2)
+    torch.cuda.synchronize()
+
+
+def long_sums(n):
+    """One expert with so many rows that a weight gradient's accumulators take long: the epilogue has to wait for them."""
+    rows = torch.ones((n, 8), dtype=torch.bfloat16, device="cuda")
+    offsets = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    w1 = torch.full((1, 8, 8), 0.125, dtype=torch.bfloat16, device="cuda")
+    w2 = torch.zeros((1, 8, 8), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    return zb.expert_ffn(rows, offsets, w1, w2, act="gelu"), w2, rows
+
+
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_gpu_usable(no_patience):
+    """Without patience the epilogue gives up at once, with the copies and products of both CTAs in flight: the kernel ends
+    by itself, the verdict names it, and the next call is right."""
+    ops.set_wait_limit(2)
+    y, w2, dy = long_sums(1 << 26)
+    want = torch.autograd.grad(y, w2, dy, retain_graph=True)[0]
+    torch.cuda.synchronize()
+    ops.check_waits()
+    for _ in range(3):
+        ops.set_wait_limit(0)
+        torch.autograd.grad(y, w2, dy, retain_graph=True)
+        torch.cuda.synchronize()
+        ops.set_wait_limit(2)
+        with pytest.raises(RuntimeError, match="wait ran out"):
+            ops.check_waits()
+        assert torch.equal(torch.autograd.grad(y, w2, dy, retain_graph=True)[0], want)
+        torch.cuda.synchronize()
+        ops.check_waits()

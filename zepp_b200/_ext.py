@@ -19,7 +19,8 @@ SYMBOLS = (
     "zepp_routed_meta", "zepp_routed_meta_noalloc", "zepp_dispatch_plan_words", "zepp_swap_decide_out_ints", "zepp_swap_decide",
     "zepp_lane_arm", "zepp_wait_geq",
     "zepp_op_gate", "zepp_op_gate_grad", "zepp_op_sort_ws_ints", "zepp_op_sort", "zepp_op_unsort", "zepp_op_unsort_grad",
-    "zepp_op_expert_ffn", "zepp_op_expert_ffn_grad", "zepp_op_grad_norm_ws_bytes", "zepp_op_grad_norm", "zepp_op_status",
+    "zepp_op_expert_ffn", "zepp_op_expert_ffn_grad", "zepp_op_grad_norm_ws_bytes", "zepp_op_grad_norm", "zepp_op_set_wait_limit_ns",
+    "zepp_op_status",
 )
 
 

@@ -55,6 +55,7 @@ constexpr int kFfnBlockBytes = 64 * 128;                // an MN-major operand b
 constexpr int kFfnStageBytes = 2 * kFfnHalfBytes;       // this CTA's features, its half of the rows
 constexpr int kFfnMaxStages = 6;
 constexpr int kFfnStagingBytes = 4096;                  // per epilogue warp: 32 rows x 32 fp32 features
+constexpr unsigned long long kFfnDrainNs = 2000000000ull;       // limit of each wait for copies and MMAs after a role gave up
 
 struct FfnArgs {
   const int* offsets;        // [G + 1]
@@ -103,6 +104,16 @@ __device__ __forceinline__ void fence_acquire_pair_shared() {
 // this thread's stores to shared memory before what the copies and MMAs do there
 __device__ __forceinline__ void fence_proxy_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long ld_shared_cluster_u64(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
 }
 // One lane of a converged warp, always the same.  The copies and MMAs take their operands from uniform registers: issued
 // under `lane == 0` they cost 570 cycles per K step on the issuing thread (380 of them without a single MMA), more than
@@ -287,6 +298,8 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
   __shared__ __align__(8) uint64_t acc_full_bar[kAccStages], acc_empty_bar[kAccStages], drain_bar;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
+  __shared__ unsigned long long s_issued;                // this CTA's loads, for a kernel that gave up
+  __shared__ uint32_t s_tail[kFfnMaxStages];             // 1 + parity on tail_bar of a load that warp 2 has yet to pass on, else 0
   extern __shared__ __align__(16) uint8_t smem_raw[];
   int* s_off = reinterpret_cast<int*>(smem_raw);         // [G + 1] first row of each group
   int* s_items = s_off + a.G + 1;                        // [G + 1] tiles before it
@@ -334,6 +347,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < stages; ++s) {
+      s_tail[s] = 0;
       mbar_init(&full_bar[s], 2);                        // one arrival (with its byte count) per CTA
       mbar_init(&empty_bar[s], 1);
       mbar_init(&tail_bar[s], 1);
@@ -371,8 +385,8 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (one per CTA)
     int stage = 0;
-    uint32_t phase = 0;
-    long long issued = 0;
+    uint32_t phase = 0, tail_phase = 0;
+    unsigned long long issued = 0;
     bool ok = true;
     for (int item = pair; item < total && ok; item += pairs) {
       const FfnTile t = ffn_tile<MODE>(a, s_off, s_items, item);
@@ -395,6 +409,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
             const int k = t.k0 + kb * 64, f = t.m0 + cta * 128;
             if (kb == t.k_steps - 1 && ffn_foreign(t.k_rows) != 0) {
               // a step with rows of other experts lands on a barrier of this CTA's own: warp 2 clears them first
+              s_tail[stage] = 1u + ((tail_phase >> stage) & 1u);
               mbar_expect_tx(&tail_bar[stage], tx);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
@@ -429,15 +444,12 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
           }
         }
         __syncwarp();
+        if (MODE == FFN_DWEIGHT && kb == t.k_steps - 1 && ffn_foreign(t.k_rows) != 0) tail_phase ^= 1u << stage;
         ++issued;
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
     }
-    if (*abortp && cta == 0 && lane == 0) {              // given up: nobody leaves before the loads have landed
-      int never = 0;
-      for (long long i = issued > stages ? issued - stages : 0; i < issued; ++i)
-        mbar_wait_bounded(&full_bar[i % stages], (uint32_t)(i / stages) & 1u, &never, a.limit_ns);
-    }
+    if (lane == 0) s_issued = issued;
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
@@ -492,12 +504,6 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
         __syncwarp();
         if (++acc == kAccStages) { acc = 0; acc_phase ^= 1; }
       }
-      if (__any_sync(0xffffffffu, *abortp)) {            // given up: nothing is in flight when TMEM is freed
-        int never = 0;
-        if (elect_one()) umma_commit_pair(&drain_bar);
-        __syncwarp();
-        mbar_wait_bounded(&drain_bar, 0, &never, a.limit_ns);
-      }
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -524,6 +530,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) {
+            s_tail[stage] = 0;
             fence_release_pair_shared();
             mbar_arrive_pair(lead_full + 8u * (uint32_t)stage);
           }
@@ -649,6 +656,34 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();                  // no MMA reads this CTA's shared memory any more, no arrival is in flight
+  // Unless a role gave up, in either CTA (both have the flag then): its partners may have issued loads and MMAs that nobody
+  // waited for.  They end before the pair leaves and frees its TMEM.
+  if (*abortp) {
+    int never = 0;
+    if (warp == 1) {
+      if (cta == 0 && elect_one()) umma_commit_pair(&drain_bar);
+      __syncwarp();
+      mbar_wait_bounded(&drain_bar, 0, &never, kFfnDrainNs);
+    }
+    if (warp == 0 && lane == 0) {
+      for (int s = 0; s < stages; ++s)
+        if (s_tail[s] != 0) mbar_wait_bounded(&tail_bar[s], s_tail[s] - 1, &never, kFfnDrainNs);
+      if (cta == 0) {
+        // All others land on this CTA's full barriers: one that lacks an arrival (a load that one CTA did not come to, or
+        // cleared rows that were not passed on) is given it, so that its phase ends with the bytes of the other.
+        const unsigned long long mine = s_issued, peer = ld_shared_cluster_u64(map_to_cta(smem_u32(&s_issued), 1u));
+        const unsigned long long most = mine > peer ? mine : peer;
+        for (unsigned long long i = most > (unsigned)stages ? most - stages : 0; i < most; ++i) {
+          const int s = (int)(i % stages);
+          if (i >= mine || s_tail[s] != 0) mbar_arrive(&full_bar[s]);
+          if (i >= peer || ld_shared_cluster_u32(map_to_cta(smem_u32(&s_tail[s]), 1u)) != 0) mbar_arrive(&full_bar[s]);
+          mbar_wait_bounded(&full_bar[s], (uint32_t)(i / stages) & 1u, &never, kFfnDrainNs);
+        }
+      }
+    }
+    __syncthreads();
+    cluster_sync_all();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);

@@ -333,6 +333,7 @@ constexpr int kPieceThreads = kPieceBytes / 16;         // consumers: a 16-byte 
 constexpr int kBulkThreads = 32 + kPieceThreads;
 constexpr int kBulkMaxStages = 16;
 constexpr int kBulkRingBytes = 48 * kPieceBytes;        // six stages, five with dy
+constexpr unsigned long long kBulkDrainNs = 2000000000ull;      // limit of each wait for copies after a role gave up
 
 struct BulkArgs {
   UnsortArgs u;
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
   const int mine = (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;      // gridDim.x <= units
   const int total = mine * per_unit;
   const long long row_bytes = a.H * (long long)sizeof(T);
+  int issued = 0;                                              // warp 0: stages whose copies it has started
 
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
@@ -382,7 +384,6 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
     // first link of every chain of loads, and one step ahead each stage still waited for most of their latency.
     int unit = blockIdx.x, step = 0, stage = 0;
     uint32_t phase = 0;
-    int issued = 0;
     int p_next = -1, p_four = -1;
     float w_next = 1.0f, w_four = 1.0f;
     auto fetch = [&](int i) {
@@ -439,11 +440,6 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
         bulk_load(st + 8 * kPieceBytes, static_cast<const unsigned char*>(a.dy) + t * row_bytes + at, bytes, &full[stage]);
       ++issued;
       if (++stage == b.stages) { stage = 0; phase ^= 1; }
-    }
-    if (*abortp) {                                             // given up: the block stays until its copies have landed
-      int never = 0;
-      for (int i = issued > b.stages ? issued - b.stages : 0; i < issued; ++i)
-        mbar_wait_bounded(&full[i % b.stages], (uint32_t)(i / b.stages) & 1u, &never, b.limit_ns);
     }
   } else {
     // ---------------------------------------------------------------- sums
@@ -547,6 +543,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
         for (long long at = v * 16; at < row_bytes; at += kPieceBytes)
           *reinterpret_cast<V*>(static_cast<unsigned char*>(a.drows) + p * row_bytes + at) = V{};
     }
+  }
+  __syncthreads();
+  if (warp == 0 && *abortp) {                                  // a role gave up: the block stays until its copies have landed
+    int never = 0;
+    for (int i = issued > b.stages ? issued - b.stages : 0; i < issued; ++i)
+      mbar_wait_bounded(&full[i % b.stages], (uint32_t)(i / b.stages) & 1u, &never, kBulkDrainNs);
   }
 }
 

@@ -2,6 +2,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <mutex>
 
@@ -22,7 +23,8 @@ using namespace zepp;
 
 // status words of the operators' bounded waits, one block per device that loads the library
 __device__ unsigned long long g_op_status[ST_WORDS];
-constexpr unsigned long long kOpWaitNs = 2000000000ull;
+// how long each of them waits (zepp_op_set_wait_limit_ns)
+std::atomic<unsigned long long> g_op_wait_ns{2000000000ull};
 
 namespace {
 
@@ -98,6 +100,12 @@ bool given(std::initializer_list<const void*> ptrs) {
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 }  // namespace
+
+extern "C" int zepp_op_set_wait_limit_ns(int64_t ns) {
+  if (ns < 0) return fail("wait limit: %lld ns", (long long)ns);
+  g_op_wait_ns = (unsigned long long)ns;
+  return 0;
+}
 
 extern "C" int zepp_op_status(void* stream, uint64_t out[8]) {
   OpDevice* d;
@@ -257,7 +265,7 @@ static bool unsort_bulk(const UnsortArgs& a, const OpDevice* d, cudaStream_t s) 
   b.stage_bytes = (GRAD ? 9 : 8) * kPieceBytes;
   b.stages = kBulkRingBytes / b.stage_bytes;
   b.status = d->status;
-  b.limit_ns = kOpWaitNs;
+  b.limit_ns = g_op_wait_ns;
   unsort_bulk_kernel<T, GRAD><<<d->sms, kBulkThreads, b.stages * b.stage_bytes, s>>>(b);
   return true;
 }
@@ -354,7 +362,7 @@ static int ffn_launch(const FfnCall& c, int64_t tiles, const CUtensorMap& f, con
   a.stages = kFfnMaxStages;
   while (ffn_smem_bytes(c.G, a.stages) > (size_t)kFfnSmemLimit) --a.stages;      // the tables of 192 groups and more take one's place
   a.status = c.dev->status;
-  a.limit_ns = kOpWaitNs;
+  a.limit_ns = g_op_wait_ns;
   const int pairs = c.dev->sms / 2;
   ffn_kernel<MODE><<<(unsigned)(tiles < pairs ? tiles : pairs) * 2, kFfnThreads, ffn_smem_bytes(c.G, a.stages), c.stream>>>(f, r32, r128, a);
   OP_LAUNCHED();

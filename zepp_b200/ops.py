@@ -44,6 +44,7 @@ _ARGS = {
     "zepp_op_expert_ffn_grad": (_P, _P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P),
     "zepp_op_grad_norm_ws_bytes": (_I,),
     "zepp_op_grad_norm": (_P, _P, _P, _I, _D, _P, _P, _P),
+    "zepp_op_set_wait_limit_ns": (_L,),
     "zepp_op_status": (_P, _P),
 }
 # a small call is bound by the host: these two cost a tenth of torch.cuda.current_device() and current_stream()
@@ -402,6 +403,14 @@ def clip_grad_norm_(tensors, max_norm):
     out = _norm(tensors, max_norm)
     torch.autograd.graph.increment_version(tensors)      # graphs that saved a tensor learn that it changed
     return out
+
+
+def set_wait_limit(seconds):
+    """How long a bounded wait of the operators' kernels lasts before the kernel gives up, for calls from now on (2 s where
+    nothing was set; captured graphs keep the limit that they were captured with)."""
+    if not 0 <= seconds <= 3600:
+        _refuse(f"a wait limit of 0..3600 seconds, got {seconds}")
+    check(_fn("zepp_op_set_wait_limit_ns")(int(seconds * 1e9)))
 
 
 def check_waits(device=None):
