@@ -213,8 +213,8 @@ int zepp_op_grad_norm(void* const* ptrs, const int64_t* sizes, const uint8_t* dt
  * zepp_op_status says so); for the calls of this process from now on, 2 s where nothing was set. */
 int zepp_op_set_wait_limit_ns(int64_t ns);
 
-/* Deferred verdict of the operators' bounded waits on the current device: synchronises `stream`, copies 8 status words
- * (as zepp_layer_status) and clears them. */
+/* Deferred verdict of the operators' bounded waits on the current device: synchronises the device, copies 8 status words
+ * (as zepp_layer_status) and, where they hold a failure, clears them. */
 int zepp_op_status(void* stream, uint64_t out[8]);
 
 #ifdef __cplusplus

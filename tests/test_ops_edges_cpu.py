@@ -1,5 +1,6 @@
 """The operators' edges that need no GPU: refusals, verdicts and sizes."""
 import pytest
+import torch
 
 import zepp_b200 as zb
 from zepp_b200 import ops
@@ -17,3 +18,64 @@ def test_wait_limit():
         with pytest.raises(AssertionError):
             ops.set_wait_limit(bad)
     ops.set_wait_limit(2)
+
+
+class Device:
+    """A device's status words: a failure is there until it is read, as zepp_op_status clears it."""
+
+    def __init__(self):
+        self.words = [0] * 8
+
+    def fail(self, what):
+        if not self.words[0]:
+            self.words = [1, what, 2, 3, 0, 0, 0, 0]
+
+    def read(self, index):
+        words, self.words = self.words, [0] * 8
+        return words
+
+
+@pytest.fixture
+def device(monkeypatch):
+    d = Device()
+    monkeypatch.setattr(ops, "_status", d.read)
+    monkeypatch.setattr(ops, "_waits", {})
+    return d
+
+
+def layer(device, status=(0,) * 8, trained=True):
+    """As much of a layer as its verdict needs."""
+    from zepp_b200.layer import EPMoE
+    l = EPMoE.__new__(EPMoE)
+    torch.nn.Module.__init__(l)
+    l.device, l._group_of, l._waits_seen, l.caps = torch.device("cuda", 0), torch.zeros(1) if trained else None, 0, None
+    l._h = type("Handle", (), {"status": lambda self: list(status)})()
+    return l
+
+
+def test_a_failed_wait_is_told_to_everybody_once(device):
+    a, b = layer(device), layer(device)
+    for l in (a, b):
+        l.check()
+    zb.check_waits(0)
+    device.fail(7)
+    for look in (a.check, lambda: zb.check_waits(0), b.check):
+        with pytest.raises(RuntimeError, match="wait id 7, item 2, step 3"):
+            look()
+        look()
+    assert ops.wait_failures(0) == 1
+    device.fail(8)
+    device.fail(9)                                       # the first one of those not yet read is kept
+    with pytest.raises(RuntimeError, match="wait id 8"):
+        zb.check_waits("cuda:0")
+    with pytest.raises(RuntimeError, match="wait id 8"):
+        b.check()
+    assert ops.wait_failures(0) == 2
+
+
+def test_a_layers_own_failure_and_the_operators_are_both_told(device):
+    device.fail(7)
+    with pytest.raises(RuntimeError, match="step failed.*wait id 5.*operator failed.*wait id 7"):
+        layer(device, status=(1, 5, 0, 0, 0, 0, 0, 0)).check()
+    with pytest.raises(RuntimeError, match="step failed"):
+        layer(device, status=(1, 5, 0, 0, 0, 0, 0, 0), trained=False).check()

@@ -82,3 +82,21 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_gpu_usable(no_patience)
         assert torch.equal(torch.autograd.grad(y, w2, dy, retain_graph=True)[0], want)
         torch.cuda.synchronize()
         ops.check_waits()
+
+
+def test_a_wait_that_runs_out_on_another_stream_is_reported(no_patience):
+    """The backward pass runs on its forward pass's stream, which is still busy when another one asks."""
+    ops.set_wait_limit(2)
+    ops.check_waits()
+    before = ops.wait_failures()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        y, w2, dy = long_sums(1 << 26)
+        torch.cuda._sleep(200_000_000)                   # about a tenth of a second before the kernel starts
+        ops.set_wait_limit(0)
+        torch.autograd.grad(y, w2, dy)
+        ops.set_wait_limit(2)
+    with pytest.raises(RuntimeError, match="wait ran out"):
+        ops.check_waits(torch.device("cuda"))
+    assert ops.wait_failures("cuda:0") == before + 1
+    ops.check_waits()

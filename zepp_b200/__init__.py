@@ -22,7 +22,8 @@ SortPlan = _ops.SortPlan
 expert_ffn = _ops.expert_ffn
 grad_norm = _ops.grad_norm
 clip_grad_norm_ = _ops.clip_grad_norm_
+check_waits = _ops.check_waits
 
 __all__ = ["SHAPES", "ModelShape", "EPMoEConfig", "tokens_per_rank", "EPMoE", "Marks", "activation", "token_buckets",
-           "route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_"]
+           "route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_", "check_waits"]
 __version__ = "0.1.0"

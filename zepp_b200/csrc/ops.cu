@@ -111,9 +111,13 @@ extern "C" int zepp_op_status(void* stream, uint64_t out[8]) {
   OpDevice* d;
   if (int rc = op_device(&d)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CU_OK(cudaDeviceSynchronize());                  // kernels of every stream record into this block
   CU_OK(cudaMemcpyAsync(out, d->status, 8 * sizeof(uint64_t), cudaMemcpyDeviceToHost, s));
-  CU_OK(cudaMemsetAsync(d->status, 0, 8 * sizeof(uint64_t), s));
   CU_OK(cudaStreamSynchronize(s));
+  if (out[ST_ERROR] != 0) {                        // without one, there is nothing to clear that a kernel could be writing
+    CU_OK(cudaMemsetAsync(d->status, 0, 8 * sizeof(uint64_t), s));
+    CU_OK(cudaStreamSynchronize(s));
+  }
   return 0;
 }
 

@@ -121,6 +121,7 @@ class EPMoE(torch.nn.Module):
         self._tokens = cfg.max_tokens_per_rank        # the bucket the next step runs at
         self._pad_bufs = {}
         self._group_of = None                         # local group of each expert (forward_train)
+        self._waits_seen = 0                          # failures of the operators' waits that check() has raised for
 
     @staticmethod
     def arena_bytes(cfg, caps):
@@ -294,6 +295,7 @@ class EPMoE(torch.nn.Module):
         assert x.shape == (topk_ids.shape[0], shape.hidden) and topk_ids.shape[1] == shape.topk, (tuple(x.shape), tuple(topk_ids.shape))
         if self._group_of is None:       # group 0 is the pad group; on one rank every expert has one slot
             self._group_of = (1 + self.placement.l2p[:, 0]).to(device=self.device, dtype=torch.int32)
+            self._waits_seen = ops._waits.get(self.device.index, (0,))[0]
         rows, plan = ops.sort_tokens(x, topk_ids.to(torch.int32), cfg.groups_per_rank, group_of=self._group_of)
         rows = ops.expert_ffn(rows, plan.offsets, self.w1, self.w2, act=shape.act)
         return ops.unsort_tokens(rows, plan, topk_weights.float())
@@ -307,18 +309,23 @@ class EPMoE(torch.nn.Module):
     # -- verdict ----------------------------------------------------------------------------
     def check(self):
         """Synchronise and raise if the last steps recorded a device-side error (a wait that ran out,
-        a capacity violation, a bad index).  The reference checks capacities on the host before it
+        a capacity violation, a bad index), or if a wait of the operators behind forward_train ran out.  The reference checks capacities on the host before it
         launches (python/zepp/comm/overlap.py:136-145); here the verdict is deferred and read on demand."""
         st = self._h.status()
+        waits = ops.wait_failures(self.device) if self._group_of is not None else 0       # forward_train ran
         if st[4]:
             dem = self._h.table("demands").cpu().tolist()
             d = Demands(*[int(v) for v in dem[:7]])
             raise CapacityExceeded(violations(d, self.caps, direct=self.cfg.comm_strategy == "direct"), d)
-        if self._group_of is not None:        # forward_train ran: its operators' waits too
-            ops.check_waits(self.device)
+        failed = []
         if st[0]:
             what = ", ".join(n for b, n in _ERR_NAMES.items() if st[0] & b)
-            raise RuntimeError(f"zepp_b200 step failed: {what} (wait id {st[1]}, peer/item {st[2]}, epoch {st[3]})")
+            failed.append(f"zepp_b200 step failed: {what} (wait id {st[1]}, peer/item {st[2]}, epoch {st[3]})")
+        if waits > self._waits_seen:
+            self._waits_seen = waits
+            failed.append(ops._wait_report(self.device.index))
+        if failed:
+            raise RuntimeError("; ".join(failed))
 
     TRACE_NAMES = ("route", "pass1", "pass1_go", "pass2", "gemm1", "gemm1_x", "gemm1_end", "gemm2", "gemm2_end",
                    "reduce", "reduce_go", "reduce_end", "scan", "scan_counts", "scan_bases", "scan_demands",

@@ -15,6 +15,7 @@ Where a backward pass is captured into a graph, make the forward pass that it be
 leaves that no graph outside of it still holds (torch runs a leaf's accumulation on the stream of the leaf's first use).
 """
 import ctypes
+import threading
 from typing import NamedTuple
 
 import numpy as np
@@ -23,7 +24,8 @@ from torch.autograd.function import once_differentiable
 
 from ._ext import check, lib
 
-__all__ = ["route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_", "check_waits"]
+__all__ = ["route_topk", "sort_tokens", "unsort_tokens", "SortPlan", "expert_ffn", "grad_norm", "clip_grad_norm_", "check_waits",
+           "wait_failures", "set_wait_limit"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SCORES = {"softmax": 0, "sigmoid": 1}
@@ -413,11 +415,48 @@ def set_wait_limit(seconds):
     check(_fn("zepp_op_set_wait_limit_ns")(int(seconds * 1e9)))
 
 
-def check_waits(device=None):
-    """Synchronise and raise if a bounded wait of an operator's kernel on `device` (default: the current one) ran out."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+_waits = {}                       # device ordinal: [failures read so far, the last one's words, those that check_waits has raised for]
+_waits_lock = threading.Lock()
+
+
+def _status(index):
+    """The operators' status words of a device; a failure is cleared there as it is read."""
     out = (ctypes.c_uint64 * 8)()
-    with torch.cuda.device(device):
-        check(_fn("zepp_op_status")(torch.cuda.current_stream().cuda_stream, ctypes.addressof(out)))
-    if out[0]:
-        raise RuntimeError(f"zepp_b200 operator failed: a device-side wait ran out (wait id {out[1]}, item {out[2]}, step {out[3]})")
+    with torch.cuda.device(index):
+        check(_fn("zepp_op_status")(_raw_stream(index), ctypes.addressof(out)))
+    return list(out)
+
+
+def _device_index(device):
+    device = torch.device("cuda" if device is None else device)
+    return _current_device() if device.index is None else device.index
+
+
+def _wait_report(index):
+    words = _waits[index][1]
+    return f"zepp_b200 operator failed: a device-side wait ran out (wait id {words[1]}, item {words[2]}, step {words[3]})"
+
+
+def wait_failures(device=None):
+    """How many times, since the process began, a look at the device (default: the current one) has found that a bounded wait
+    of an operator's kernel had run out; looks once more first, after synchronising the device.  Nobody's look takes a
+    failure away from another: each compares the count with its own last one."""
+    index = _device_index(device)
+    with _waits_lock:
+        words = _status(index)
+        seen = _waits.setdefault(index, [0, None, 0])
+        if words[0]:
+            seen[0] += 1
+            seen[1] = words
+        return seen[0]
+
+
+def check_waits(device=None):
+    """Synchronise the device (default: the current one) and raise if a bounded wait of an operator's kernel on it, on any
+    stream, has run out since the last check_waits: outputs of the calls in between may be incomplete."""
+    index = _device_index(device)
+    count = wait_failures(index)
+    seen = _waits[index]
+    if count > seen[2]:
+        seen[2] = count
+        raise RuntimeError(_wait_report(index))
