@@ -100,3 +100,21 @@ def test_a_wait_that_runs_out_on_another_stream_is_reported(no_patience):
         ops.check_waits(torch.device("cuda"))
     assert ops.wait_failures("cuda:0") == before + 1
     ops.check_waits()
+
+
+def test_a_long_sum_is_waited_for(no_patience):
+    """The epilogue's wait for a sum over all rows of an expert grows with their number: it does not run out because there
+    are many.  2^26 rows are 2^20 steps, for which the limit is twice what was set."""
+    ops.set_wait_limit(2)
+    y, w2, dy = long_sums(1 << 26)
+    torch.autograd.grad(y, w2, dy, retain_graph=True)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    want = torch.autograd.grad(y, w2, dy, retain_graph=True)[0]
+    end.record()
+    torch.cuda.synchronize()
+    ops.check_waits()
+    ops.set_wait_limit(0.7 * start.elapsed_time(end) / 1e3)
+    got = torch.autograd.grad(y, w2, dy)[0]
+    ops.check_waits()
+    assert torch.equal(got, want)

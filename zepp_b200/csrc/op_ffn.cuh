@@ -568,7 +568,9 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
       }
       int got = 1;
       if (lane == 0) {
-        got = mbar_wait_bounded(&acc_full_bar[acc], acc_phase, abortp, a.limit_ns) ? 1 : 0;
+        // the one wait that is as long as a sum (0.28 us a step: 2 s would be 460 million rows): 2^-20 of the limit more per step
+        const unsigned long long limit = a.limit_ns + (a.limit_ns >> 20) * (unsigned long long)t.k_steps;
+        got = mbar_wait_bounded(&acc_full_bar[acc], acc_phase, abortp, limit) ? 1 : 0;
         if (!got && !*abortp) give_up(WAIT_TMEM_FULL, item, acc);
       }
       got = __shfl_sync(0xffffffffu, got, 0);
