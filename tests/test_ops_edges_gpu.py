@@ -102,11 +102,13 @@ def test_a_wait_that_runs_out_on_another_stream_is_reported(no_patience):
     ops.check_waits()
 
 
-def test_a_long_sum_is_waited_for(no_patience):
+@pytest.mark.parametrize("spare", (0, 3))
+def test_a_long_sum_is_waited_for(no_patience, spare):
     """The epilogue's wait for a sum over all rows of an expert grows with their number: it does not run out because there
-    are many.  2^26 rows are 2^20 steps, for which the limit is twice what was set."""
+    are many.  2^26 rows are 2^20 steps, for which the limit is twice what was set.  With three rows more the last
+    step holds rows behind the expert's, whose clearing waits as long."""
     ops.set_wait_limit(2)
-    y, w2, dy = long_sums(1 << 26)
+    y, w2, dy = long_sums((1 << 26) + spare)
     torch.autograd.grad(y, w2, dy, retain_graph=True)
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     start.record()

@@ -286,6 +286,11 @@ __device__ __forceinline__ FfnTile ffn_tile(const FfnArgs& a, const int* s_off, 
   }
   return t;
 }
+// The limit of a wait that lasts as long as `steps` steps of sums (0.28 us each with one tile on the machine: 2 s would be 460
+// million rows): 2^-20 of what was set more for each.  All other waits are for a step or two.
+__device__ __forceinline__ unsigned long long ffn_limit(const FfnArgs& a, unsigned long long steps) {
+  return a.limit_ns + (a.limit_ns >> 20) * steps;
+}
 // rows of the last K step of a weight gradient that an instruction would read but that belong to other experts
 __device__ __forceinline__ int ffn_foreign(int rows) { return (16 - (rows & 15)) & 15; }
 
@@ -511,13 +516,16 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
     if (MODE == FFN_DWEIGHT) {
       int stage = 0;
       uint32_t tail_phase = 0;
+      unsigned long long steps = 0;                      // since the last wait
       for (int item = pair; item < total; item += pairs) {
         const FfnTile t = ffn_tile<MODE>(a, s_off, s_items, item);
         const int foreign = ffn_foreign(t.k_rows);
         if (t.k_steps == 0) continue;
         stage = (stage + t.k_steps - 1) % stages;
+        steps += t.k_steps;
         if (foreign != 0) {
-          const bool ok = mbar_wait_bounded(&tail_bar[stage], (tail_phase >> stage) & 1u, abortp, a.limit_ns);
+          const bool ok = mbar_wait_bounded(&tail_bar[stage], (tail_phase >> stage) & 1u, abortp, ffn_limit(a, steps));
+          steps = 0;
           if (!__all_sync(0xffffffffu, ok)) {
             if (lane == 0) give_up(WAIT_MBAR_FULL, item, -1);
             break;
@@ -568,9 +576,7 @@ ffn_kernel(const __grid_constant__ CUtensorMap tm_f, const __grid_constant__ CUt
       }
       int got = 1;
       if (lane == 0) {
-        // the one wait that is as long as a sum (0.28 us a step: 2 s would be 460 million rows): 2^-20 of the limit more per step
-        const unsigned long long limit = a.limit_ns + (a.limit_ns >> 20) * (unsigned long long)t.k_steps;
-        got = mbar_wait_bounded(&acc_full_bar[acc], acc_phase, abortp, limit) ? 1 : 0;
+        got = mbar_wait_bounded(&acc_full_bar[acc], acc_phase, abortp, ffn_limit(a, t.k_steps)) ? 1 : 0;
         if (!got && !*abortp) give_up(WAIT_TMEM_FULL, item, acc);
       }
       got = __shfl_sync(0xffffffffu, got, 0);
