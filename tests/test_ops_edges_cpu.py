@@ -79,3 +79,11 @@ def test_a_layers_own_failure_and_the_operators_are_both_told(device):
         layer(device, status=(1, 5, 0, 0, 0, 0, 0, 0)).check()
     with pytest.raises(RuntimeError, match="step failed"):
         layer(device, status=(1, 5, 0, 0, 0, 0, 0, 0), trained=False).check()
+
+
+@pytest.mark.parametrize("tokens, k", [(1 << 62, 4), ((1 << 61) + 1, 8), ((1 << 58) + 5, 64), (1 << 31, 1)])
+def test_token_counts_whose_product_wraps_are_refused(tokens, k):
+    for rc in (ops._fn("zepp_op_sort")(None, 0, tokens, k, 8, None, None, 0, 8, None, None, None, None, None),
+               ops._fn("zepp_op_unsort")(None, 0, tokens, k, 8, None, None, None, None),
+               ops._fn("zepp_op_unsort_grad")(None, None, 0, tokens, k, 8, 8, None, None, None, None, None, None)):
+        assert "32-bit" in error(rc)

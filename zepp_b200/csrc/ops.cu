@@ -191,7 +191,7 @@ extern "C" int zepp_op_gate_grad(const void* logits, int dtype, int64_t T, int G
 static int sort_check(const char* what, int dtype, int64_t T, int K, int64_t H) {
   if (dtype < OP_F32 || dtype > OP_F16) return fail("%s: unknown element type %d", what, dtype);
   if (K < 1 || K > 64) return fail("%s: top-k of 1..64 (got %d)", what, K);
-  if (T < 0 || T * K >= (1ll << 31)) return fail("%s: %lld tokens x %d copies do not fit 32-bit row numbers", what, (long long)T, K);
+  if (T < 0 || T >= (1ll << 31) || T * K >= (1ll << 31)) return fail("%s: %lld tokens x %d copies do not fit 32-bit row numbers", what, (long long)T, K);
   if (H < 1 || H > (1 << 20)) return fail("%s: rows of 1..%d elements (got %lld)", what, 1 << 20, (long long)H);
   return 0;
 }
