@@ -46,6 +46,16 @@ def test_expert_ffn_rows_of_neighbours_never_reach_a_weight_gradient(act, expert
     ops.check_waits()
 
 
+# ------------------------------------------------------------------------------------------------ sort by expert and back
+def test_sort_with_an_empty_group_table():
+    """No id has a group in it, so no copy gets a row."""
+    x = randn((5, 16), gen(1)).requires_grad_(True)
+    ids = torch.arange(10, dtype=torch.int32, device="cuda").view(5, 2) % 4
+    rows, plan = zb.sort_tokens(x, ids, 4, group_of=torch.empty(0, dtype=torch.int32, device="cuda"))
+    assert not plan.offsets.any() and bool((plan.position == -1).all()) and not rows.any()
+    assert not torch.autograd.grad(rows, x, torch.ones_like(rows))[0].any()
+
+
 # ------------------------------------------------------------------------------------------------- waits that run out
 @pytest.fixture
 def no_patience():

@@ -238,7 +238,8 @@ def sort_tokens(x, ids, num_experts, group_of=None):
     if group_of is not None:
         if group_of.dim() != 1 or group_of.dtype != torch.int32:
             _refuse("group_of: a table of int32")
-        group_of = group_of.contiguous()
+        # an empty table has no address, which would stand for no table at all
+        group_of = group_of.contiguous() if group_of.shape[0] else group_of.new_full((1,), -1)
     _on(x.device, ids, group_of)
     args = (x.contiguous(), ids.contiguous(), int(num_experts), group_of)
     rows, offsets, position = _Sort.apply(*args) if x.requires_grad and torch.is_grad_enabled() else _sort(*args)
