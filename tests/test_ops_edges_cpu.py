@@ -87,3 +87,12 @@ def test_token_counts_whose_product_wraps_are_refused(tokens, k):
                ops._fn("zepp_op_unsort")(None, 0, tokens, k, 8, None, None, None, None),
                ops._fn("zepp_op_unsort_grad")(None, None, 0, tokens, k, 8, 8, None, None, None, None, None, None)):
         assert "32-bit" in error(rc)
+
+
+def test_clipping_refuses_parameters():
+    """It scales what it is given: parameters instead of their gradients would be shrunk."""
+    p = torch.nn.Parameter(torch.ones(3))
+    for tensors in ([p], [torch.ones(3), p], (q for q in (p,))):
+        with pytest.raises(AssertionError, match="leaf"):
+            zb.clip_grad_norm_(tensors, 1.0)
+    assert bool((p == 1).all())

@@ -130,3 +130,16 @@ def test_a_long_sum_is_waited_for(no_patience, spare):
     got = torch.autograd.grad(y, w2, dy)[0]
     ops.check_waits()
     assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------------------------------------- norm of many, clipping
+def test_clipping_takes_gradients_and_no_parameters():
+    p = torch.nn.Parameter(torch.full((50,), 2.0, device="cuda"))
+    with pytest.raises(AssertionError, match="leaf"):
+        zb.clip_grad_norm_([p], 1.0)
+    assert bool((p == 2).all())
+    grads = torch.autograd.grad(p.square().sum(), p, create_graph=True)       # of a graph, but not a leaf
+    zb.clip_grad_norm_(grads, 1.0)
+    # 50 squares of 4: norm 4 sqrt(50); the factor, the product and the root round once each
+    assert bool(((grads[0].detach().double() * 50 ** 0.5 - 1).abs() <= 4 * 2.0 ** -24 + 1e-6).all())
+    assert float(zb.grad_norm([p])) > 0                                       # only reads

@@ -397,12 +397,15 @@ def grad_norm(tensors):
 @torch.no_grad()
 def clip_grad_norm_(tensors, max_norm):
     """Scale the tensors in place by min(1, max_norm / (norm + 1e-6)), norm being grad_norm(tensors), which is returned.
+    The tensors are the gradients themselves, not parameters: leaves that require a gradient are refused.
     With a norm of NaN every element becomes NaN; with an infinite one the finite elements become 0.  The tensors must not
     overlap; other orders of their dimensions are fine, gaps are not."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         _refuse(f"max_norm: not negative, got {max_norm}")
     tensors = list(tensors)
+    if any([t.requires_grad and t.is_leaf for t in tensors]):
+        _refuse("gradients, not the parameters that they belong to: a tensor is a leaf that requires a gradient")
     out = _norm(tensors, max_norm)
     torch.autograd.graph.increment_version(tensors)      # graphs that saved a tensor learn that it changed
     return out
