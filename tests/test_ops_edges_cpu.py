@@ -48,6 +48,7 @@ def layer(device, status=(0,) * 8, trained=True):
     from zepp_b200.layer import EPMoE
     l = EPMoE.__new__(EPMoE)
     torch.nn.Module.__init__(l)
+    l.w1 = l.w2 = None
     l.device, l._group_of, l._waits_seen, l.caps = torch.device("cuda", 0), torch.zeros(1) if trained else None, 0, None
     l._h = type("Handle", (), {"status": lambda self: list(status)})()
     return l
@@ -96,3 +97,12 @@ def test_clipping_refuses_parameters():
         with pytest.raises(AssertionError, match="leaf"):
             zb.clip_grad_norm_(tensors, 1.0)
     assert bool((p == 1).all())
+
+
+def test_clipping_a_layer_without_gradients(device):
+    l = layer(device)
+    l.device = torch.device("cpu")
+    for w, others in ((None, ()), (torch.zeros(2, requires_grad=True), [torch.zeros(3, requires_grad=True)])):
+        l.w1 = l.w2 = w
+        norm = l.clip_grad_norm_(1.0, others=others)
+        assert norm.shape == () and norm.dtype == torch.float32 and float(norm) == 0.0

@@ -302,9 +302,13 @@ class EPMoE(torch.nn.Module):
 
     def clip_grad_norm_(self, max_norm, others=()):
         """Scale the gradients of the expert weights and of `others` (parameters, such as the router's) in place to at
-        most max_norm together; returns their norm.  Parameters without a gradient are left out."""
+        most max_norm together; returns their norm.  Parameters without a gradient are left out; without any gradient the
+        norm is 0."""
         params = [p for p in (self.w1, self.w2, *others) if p is not None]
-        return ops.clip_grad_norm_([p.grad for p in params if p.grad is not None], max_norm)
+        grads = [p.grad for p in params if p.grad is not None]
+        if not grads:
+            return torch.zeros((), dtype=torch.float32, device=self.device)
+        return ops.clip_grad_norm_(grads, max_norm)
 
     # -- verdict ----------------------------------------------------------------------------
     def check(self):
