@@ -1,4 +1,6 @@
 """The operators' edges that need no GPU: refusals, verdicts and sizes."""
+import collections
+
 import pytest
 import torch
 
@@ -43,12 +45,16 @@ def device(monkeypatch):
     return d
 
 
+Config = collections.namedtuple("Config", "ranks swap")
+
+
 def layer(device, status=(0,) * 8, trained=True):
     """As much of a layer as its verdict needs."""
     from zepp_b200.layer import EPMoE
     l = EPMoE.__new__(EPMoE)
     torch.nn.Module.__init__(l)
     l.w1 = l.w2 = None
+    l.cfg = Config(ranks=1, swap=False)
     l.device, l._group_of, l._waits_seen, l.caps = torch.device("cuda", 0), torch.zeros(1) if trained else None, 0, None
     l._h = type("Handle", (), {"status": lambda self: list(status)})()
     return l
@@ -106,3 +112,14 @@ def test_clipping_a_layer_without_gradients(device):
         l.w1 = l.w2 = w
         norm = l.clip_grad_norm_(1.0, others=others)
         assert norm.shape == () and norm.dtype == torch.float32 and float(norm) == 0.0
+
+
+@pytest.mark.parametrize("ranks, swap", [(2, False), (1, True), (8, True)])
+def test_training_calls_are_for_one_rank_without_swap(device, ranks, swap):
+    l = layer(device)
+    l.w1, l.w2 = torch.zeros(2), torch.zeros(2)
+    l.cfg = Config(ranks, swap)
+    for call in (l.train_weights, lambda: l.forward_train(None, None, None), lambda: l.clip_grad_norm_(1.0)):
+        with pytest.raises(AssertionError, match="one rank, without swap"):
+            call()
+    assert not l.w1.requires_grad and not l.w2.requires_grad

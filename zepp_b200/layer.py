@@ -278,9 +278,14 @@ class EPMoE(torch.nn.Module):
         assert logits.dim() == 2 and logits.shape[1] == self.cfg.shape.num_experts, tuple(logits.shape)
         return ops.route_topk(logits, self.cfg.shape.topk, score=score, renormalize=renormalize, bias=bias, scale=scale)
 
+    def _one_rank(self, what):
+        assert self.cfg.ranks == 1 and not self.cfg.swap, f"{what}: layers of one rank, without swap"
+
     def train_weights(self):
         """The expert weights as leaves that take gradients: [w1 [groups, ffn1, H], w2 [groups, H, ffn]], the tensors that
-        step() reads, so an optimizer that updates them in place serves both.  Unused slots get zero gradients."""
+        step() reads, so an optimizer that updates them in place serves both.  Unused slots get zero gradients.  Layers of one
+        rank, without swap: elsewhere an expert has several copies, or moves."""
+        self._one_rank("train_weights")
         assert self.w1 is not None, "load_weights / set_weights first"
         return [self.w1.requires_grad_(True), self.w2.requires_grad_(True)]
 
@@ -290,7 +295,7 @@ class EPMoE(torch.nn.Module):
         without swap.  Agrees with step() to bf16 rounding: the activations and the weighted sum keep fp32 where step()
         rounds as the reference does."""
         cfg, shape = self.cfg, self.cfg.shape
-        assert cfg.ranks == 1 and not cfg.swap, "forward_train: layers of one rank, without swap"
+        self._one_rank("forward_train")
         assert self.w1 is not None, "load_weights / set_weights first"
         assert x.shape == (topk_ids.shape[0], shape.hidden) and topk_ids.shape[1] == shape.topk, (tuple(x.shape), tuple(topk_ids.shape))
         if self._group_of is None:       # group 0 is the pad group; on one rank every expert has one slot
@@ -303,7 +308,8 @@ class EPMoE(torch.nn.Module):
     def clip_grad_norm_(self, max_norm, others=()):
         """Scale the gradients of the expert weights and of `others` (parameters, such as the router's) in place to at
         most max_norm together; returns their norm.  Parameters without a gradient are left out; without any gradient the
-        norm is 0."""
+        norm is 0.  Layers of one rank, without swap: there is no sum over ranks."""
+        self._one_rank("clip_grad_norm_")
         params = [p for p in (self.w1, self.w2, *others) if p is not None]
         grads = [p.grad for p in params if p.grad is not None]
         if not grads:
