@@ -45,7 +45,7 @@ def device(monkeypatch):
     return d
 
 
-Config = collections.namedtuple("Config", "ranks swap")
+Config = collections.namedtuple("Config", "ranks swap shape", defaults=(None,))
 
 
 def layer(device, status=(0,) * 8, trained=True):
