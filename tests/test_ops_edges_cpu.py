@@ -3,6 +3,7 @@ import collections
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import zepp_b200 as zb
 from zepp_b200 import ops
@@ -123,3 +124,14 @@ def test_training_calls_are_for_one_rank_without_swap(device, ranks, swap):
         with pytest.raises(AssertionError, match="one rank, without swap"):
             call()
     assert not l.w1.requires_grad and not l.w2.requires_grad
+
+
+def test_tensors_with_a_tangent():
+    t = torch.ones(3)
+    with fwAD.dual_level():
+        d = fwAD.make_dual(t, t)
+        ops._no_tangents(t, None, torch.zeros(2, dtype=torch.int32))
+        for some in ((d,), (t, d), (None, d)):
+            with pytest.raises(AssertionError, match="tangent"):
+                ops._no_tangents(*some)
+    ops._no_tangents(t, d)

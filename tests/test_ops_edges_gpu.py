@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import zepp_b200 as zb
 from zepp_b200 import ops
@@ -143,3 +144,31 @@ def test_clipping_takes_gradients_and_no_parameters():
     # 50 squares of 4: norm 4 sqrt(50); the factor, the product and the root round once each
     assert bool(((grads[0].detach().double() * 50 ** 0.5 - 1).abs() <= 4 * 2.0 ** -24 + 1e-6).all())
     assert float(zb.grad_norm([p])) > 0                                       # only reads
+
+
+# ------------------------------------------------------------------------------------------------- forward-mode derivatives
+def test_inputs_with_a_tangent_are_refused():
+    """A dual tensor does not require a gradient; its tangent would be dropped, which is a derivative of zero."""
+    i32, bf = dict(dtype=torch.int32, device="cuda"), dict(dtype=torch.bfloat16, device="cuda")
+    l, x, w = (torch.rand(*s, device="cuda") for s in ((4, 8), (4, 16), (4, 2)))
+    ids = torch.arange(8, **i32).view(4, 2)
+    rows, plan = zb.sort_tokens(x, ids, 8)
+    a, w1, w2, off = torch.rand(4, 16, **bf), torch.rand(2, 16, 16, **bf), torch.rand(2, 16, 8, **bf), torch.tensor([0, 1, 4], **i32)
+    calls = [(lambda l: zb.route_topk(l, 2), (l,)), (lambda x: zb.sort_tokens(x, ids, 8), (x,)),
+             (lambda r, w: zb.unsort_tokens(r, plan, w), (rows, w)), (lambda a, u, v: zb.expert_ffn(a, off, u, v), (a, w1, w2)),
+             (lambda t: zb.grad_norm([l, t]), (x,)), (lambda t: zb.clip_grad_norm_([l, t], 1.0), (x,))]
+    for call, args in calls:
+        kept = [t.clone() for t in args]
+        with fwAD.dual_level():
+            for i in range(len(args)):
+                with pytest.raises(AssertionError, match="tangent"):
+                    call(*[fwAD.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)])
+            call(*args)                                                           # without a tangent
+        if call is not calls[-1][0]:
+            assert all(torch.equal(t, k) for t, k in zip(args, kept))
+    with fwAD.dual_level(), pytest.raises((AssertionError, RuntimeError)):        # as well as a gradient: still no silent zero
+        zb.unsort_tokens(fwAD.make_dual(rows, torch.ones_like(rows)), plan, w.requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: zb.route_topk(t, 2)[1])(l[None].expand(3, 4, 8))
+    with pytest.raises((AssertionError, RuntimeError)):
+        torch.func.jvp(lambda t: zb.route_topk(t, 2)[1], (l,), (torch.ones_like(l),))

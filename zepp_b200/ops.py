@@ -9,7 +9,8 @@
 Each call is one to five kernels of libzepp_b200.so on the current stream of its tensors' device; nothing is read back
 on the host, and calls can be captured into CUDA graphs after one call on that device outside of a capture.  Arguments
 that do not fit are refused with an AssertionError, as everywhere in this package.  Inputs that are not contiguous (or,
-for expert_ffn, not on a 16-byte boundary) are copied.  Gradients are first derivatives only.
+for expert_ffn, not on a 16-byte boundary) are copied.  Gradients are first derivatives only, and there are no forward-mode
+derivatives: inputs that have a tangent are refused.
 
 Where a backward pass is captured into a graph, make the forward pass that it belongs to inside the same capture, of
 leaves that no graph outside of it still holds (torch runs a leaf's accumulation on the stream of the leaf's first use).
@@ -20,6 +21,7 @@ from typing import NamedTuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._ext import check, lib
@@ -91,6 +93,14 @@ def _on(device, *tensors):
             _refuse(f"a tensor is on {t.device}, not on {device} as the first one")
 
 
+def _no_tangents(*tensors):
+    """The kernels compute values only: of a dual tensor of forward-mode derivatives they would drop the tangent."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse("forward-mode derivatives: a tensor has a tangent, and the operators have gradients only")
+
+
 def _first_derivative(backward):
     """once_differentiable, whose own cost (4 us) is paid only where a graph of the gradients is wanted"""
     slow = once_differentiable(backward)
@@ -151,6 +161,7 @@ def route_topk(logits, k, score="softmax", renormalize=True, bias=None, scale=1.
             _refuse("bias: float32 [experts], with sigmoid scores")
         _on(logits.device, bias)
         bias = bias.detach().contiguous()
+    _no_tangents(logits)
     logits = logits.contiguous()
     args = (logits, int(k), _SCORES[score], int(bool(renormalize)), bias, float(scale))
     return _Gate.apply(*args) if logits.requires_grad and torch.is_grad_enabled() else _gate(*args)
@@ -241,6 +252,7 @@ def sort_tokens(x, ids, num_experts, group_of=None):
         # an empty table has no address, which would stand for no table at all
         group_of = group_of.contiguous() if group_of.shape[0] else group_of.new_full((1,), -1)
     _on(x.device, ids, group_of)
+    _no_tangents(x)
     args = (x.contiguous(), ids.contiguous(), int(num_experts), group_of)
     rows, offsets, position = _Sort.apply(*args) if x.requires_grad and torch.is_grad_enabled() else _sort(*args)
     return rows, SortPlan(offsets, position)
@@ -260,6 +272,7 @@ def unsort_tokens(rows, plan, weights=None):
             _refuse(f"weights: float32 [{T}, {K}], got {tuple(weights.shape)} {weights.dtype}")
         weights = weights.contiguous()
     _on(rows.device, plan.position, plan.offsets, weights)
+    _no_tangents(rows, weights)
     rows = rows.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _Unsort.apply(rows, plan.offsets.contiguous(), plan.position.contiguous(), weights)
@@ -327,6 +340,7 @@ def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
     if H % 8 or I % 8 or H < 8 or I < 8 or not 1 <= G <= MAX_FFN_EXPERTS:
         _refuse(f"hidden and ffn are multiples of 8, 1..{MAX_FFN_EXPERTS} experts, got {H}, {I}, {G}")
     _on(rows.device, offsets, w1, w2)
+    _no_tangents(rows, w1, w2)
     args = (_dense16(rows), offsets.contiguous(), _dense16(w1), _dense16(w2), _ACTS[act])
     if torch.is_grad_enabled() and (rows.requires_grad or w1.requires_grad or w2.requires_grad):
         return _ExpertFFN.apply(*args)
@@ -355,6 +369,7 @@ def _norm(tensors, max_norm):
         _refuse("CUDA tensors of one device, of float32, bfloat16 or float16")
     if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.is_contiguous() or _is_dense(t) for t in tensors):
         _refuse("tensors whose elements lie without gaps and only once in memory")
+    _no_tangents(*tensors)
     n = len(tensors)
     out = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(_fn("zepp_op_grad_norm_ws_bytes")(n), dtype=torch.uint8, device=device)
