@@ -146,6 +146,20 @@ def test_clipping_takes_gradients_and_no_parameters():
     assert float(zb.grad_norm([p])) > 0                                       # only reads
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size, max_norm", [(1e38, 1.0), (1e38, 1e-3), (3e38, 1e-6), (1e38, 1e-9), (3e38, 30.0)])
+def test_clipping_by_factors_below_the_normal_numbers(dtype, size, max_norm):
+    """Elements near the top of the range: the factor has fewer bits than fp32's normal numbers, the result has all."""
+    t = (torch.rand(1000, generator=gen(7), device="cuda") * size).to(dtype)
+    want = t.double()
+    total = float(want.norm())
+    want = want * min(1.0, max_norm / (total + 1e-6))
+    zb.clip_grad_norm_([t], max_norm)
+    # sums of at most 64 squares in fp32 (half of it in the root), the quotient, the product and the result's own rounding
+    bound = (torch.finfo(dtype).eps / 2 + 40 * 2.0 ** -24) * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((t.double() - want).abs() <= bound).all())
+
+
 # ------------------------------------------------------------------------------------------------- forward-mode derivatives
 def test_inputs_with_a_tangent_are_refused():
     """A dual tensor does not require a gradient; its tangent would be dropped, which is a derivative of zero."""

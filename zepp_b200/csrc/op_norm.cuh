@@ -106,6 +106,18 @@ __device__ __forceinline__ void norm_scale(T* base, long long head, long long en
   }
 }
 
+// The same with a factor below the normal numbers of fp32 (a norm beyond 1e38 of the limit), which would hold fewer bits of it
+// the smaller it is.
+template <typename T>
+__device__ __noinline__ void norm_scale_wide(T* base, long long head, long long end, long long first, double c) {
+  constexpr int E = 16 / (int)sizeof(T);
+  for (int q = 0; q < kNormVecs; ++q) {
+    const long long e0 = first + (long long)(q * kNormThreads + threadIdx.x) * E;
+    for (int i = 0; i < E; ++i)
+      if (e0 + i >= head && e0 + i < end) base[e0 + i] = from_f32<T>((float)((double)to_f32<T>(base[e0 + i]) * c));
+  }
+}
+
 template <int CAP>
 __device__ __forceinline__ int norm_tensor_of(const NormTable<CAP>& t, int chunk) {
   int lo = 0, hi = t.count - 1;
@@ -164,6 +176,19 @@ norm_scale_kernel(const __grid_constant__ NormTable<CAP> t, const double* partia
   const double ratio = max_norm / (total + 1e-6);
   const float c = (float)(ratio > 1.0 ? 1.0 : ratio);      // NaN stays NaN
   if (c == 1.0f) return;
+  if (ratio > 0.0 && ratio < 1.17549435e-38) {
+    for (int i = blockIdx.x; i < t.chunk0[t.count]; i += gridDim.x) {
+      const int k = norm_tensor_of(t, i);
+      const long long bytes = (long long)(i - t.chunk0[k]) * kNormChunkBytes;
+      if (t.type[k] == OP_F32)
+        norm_scale_wide<float>(reinterpret_cast<float*>(t.base[k]), t.head[k], t.end[k], bytes / 4, ratio);
+      else if (t.type[k] == OP_BF16)
+        norm_scale_wide<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(t.base[k]), t.head[k], t.end[k], bytes / 2, ratio);
+      else
+        norm_scale_wide<__half>(reinterpret_cast<__half*>(t.base[k]), t.head[k], t.end[k], bytes / 2, ratio);
+    }
+    return;
+  }
   for (int i = blockIdx.x; i < t.chunk0[t.count]; i += gridDim.x) {
     const int chunk = t.chunk0[t.count] - 1 - i;
     const int k = norm_tensor_of(t, chunk);
