@@ -160,6 +160,19 @@ def test_clipping_by_factors_below_the_normal_numbers(dtype, size, max_norm):
     assert bool(((t.double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("special", [1.0, math.inf, -math.inf, math.nan])
+def test_clipping_with_an_infinite_limit(special):
+    """No limit: nothing changes, whatever the norm, but for a norm of NaN."""
+    t = randn((500,), gen(3))
+    t[17] = special
+    kept = t.clone()
+    norm = zb.clip_grad_norm_([t], math.inf)
+    if math.isnan(special):
+        assert math.isnan(float(norm)) and bool(t.isnan().all())
+    else:
+        assert torch.equal(t, kept) and math.isinf(float(norm)) == math.isinf(special)
+
+
 # ------------------------------------------------------------------------------------------------- forward-mode derivatives
 def test_inputs_with_a_tangent_are_refused():
     """A dual tensor does not require a gradient; its tangent would be dropped, which is a derivative of zero."""

@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(kNormThreads)
 norm_scale_kernel(const __grid_constant__ NormTable<CAP> t, const double* partials, int n, double max_norm, float* out) {
   const double total = norm_total(partials, n);
   if (blockIdx.x == 0 && threadIdx.x == 0 && out != nullptr) *out = (float)total;
-  const double ratio = max_norm / (total + 1e-6);
+  // without a limit nothing changes, elements that are infinite neither
+  const double ratio = max_norm == INFINITY && total == INFINITY ? 1.0 : max_norm / (total + 1e-6);
   const float c = (float)(ratio > 1.0 ? 1.0 : ratio);      // NaN stays NaN
   if (c == 1.0f) return;
   if (ratio > 0.0 && ratio < 1.17549435e-38) {

@@ -413,8 +413,9 @@ def grad_norm(tensors):
 def clip_grad_norm_(tensors, max_norm):
     """Scale the tensors in place by min(1, max_norm / (norm + 1e-6)), norm being grad_norm(tensors), which is returned.
     The tensors are the gradients themselves, not parameters: leaves that require a gradient are refused.
-    With a norm of NaN every element becomes NaN; with an infinite one the finite elements become 0.  The tensors must not
-    overlap; other orders of their dimensions are fine, gaps are not."""
+    With a norm of NaN every element becomes NaN; where an element is infinite, the finite ones become 0 and the infinite ones
+    NaN; with an infinite max_norm only NaN changes anything.  The tensors must not overlap; other orders of their dimensions
+    are fine, gaps are not."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         _refuse(f"max_norm: not negative, got {max_norm}")
