@@ -19,6 +19,85 @@ def randn(shape, g, dtype=torch.float32, std=1.0):
     return (torch.randn(shape, generator=g, device="cuda") * std).to(dtype)
 
 
+def same_places(got, want):
+    """NaN, +inf and -inf in the same places."""
+    return (torch.equal(got.isnan(), want.isnan()) and torch.equal(got == math.inf, want == math.inf)
+            and torch.equal(got == -math.inf, want == -math.inf))
+
+
+# ------------------------------------------------------------------------------------------------------------- gate
+@pytest.mark.parametrize("G, k", [(40, 4), (128, 8), (384, 8), (1000, 32)])
+@pytest.mark.parametrize("score, renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gate_gradient_of_rows_with_nan(G, k, score, renormalize, dtype):
+    """A row's NaN makes its weights NaN and with them the gradients of the experts that it chose, or of all experts where
+    the weights are probabilities over all of them; it reaches no other row.  What is masked with -inf besides stays out."""
+    g = gen(G + k)
+    clean, dw = randn((12, G), g, dtype, 2.0), randn((12, k), g)
+    l = clean.clone()
+    l[1, 5] = math.nan                                # one
+    l[4] = math.nan                                   # nothing else
+    l[7, 2], l[7, 3:] = math.nan, -math.inf           # two experts left to choose
+    res = []
+    for t in (clean, l):
+        t = t.clone().requires_grad_(True)
+        ids, w = zb.route_topk(t, k, score=score, renormalize=renormalize)
+        res.append((ids, w.detach(), torch.autograd.grad(w, t, dw)[0]))
+    (_, w0, d0), (ids, w, d) = res
+    bad = torch.tensor([1, 4, 7], device="cuda")
+    good = torch.tensor([i for i in range(12) if i not in (1, 4, 7)], device="cuda")
+    assert torch.equal(w[good], w0[good]) and torch.equal(d[good], d0[good]) and bool(w[bad].isnan().all())
+    assert bool((ids[1] != 5).all()) and bool((ids[4] == -1).all()) and sorted(ids[7].tolist())[-2:] == [0, 1] and bool((ids[7, 2:] == -1).all())
+    want = torch.zeros((12, G), device="cuda")
+    if score == "softmax" and not renormalize:
+        want[bad] = math.nan
+    else:
+        want[1, ids[1].long()] = math.nan
+        want[7, :2] = math.nan
+    assert same_places(d[bad].float(), want[bad]) and bool((d[bad].nan_to_num(0.0) == 0).all())
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gate_of_rows_with_an_infinite_logit(score):
+    """+inf is chosen first.  Its sigmoid is 1 with slope 0; its softmax is inf - inf."""
+    l = randn((3, 20), gen(1))
+    l[1, 6] = math.inf
+    l.requires_grad_(True)
+    ids, w = zb.route_topk(l, 3, score=score, renormalize=False)
+    d = torch.autograd.grad(w, l, torch.ones_like(w))[0]
+    assert int(ids[1, 0]) == 6 and bool(w[::2].isfinite().all()) and bool(d[::2].isfinite().all())
+    if score == "sigmoid":
+        assert float(w.detach()[1, 0]) == 1.0 and float(d[1, 6]) == 0.0 and bool(d[1].isfinite().all())
+    else:
+        assert bool(w[1, 0].isnan()) and bool(d[1, 6].isnan())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_infinities_keep_their_sign(dtype):
+    """Rows, sums and gradients that are infinite: the same sign as by the formulas."""
+    g = gen(5)
+    T, K, H = 30, 4, 64
+    ids = torch.randint(0, 6, (T, K), generator=g, device="cuda", dtype=torch.int32)
+    x = randn((T, H), g, dtype)
+    x[3, 5], x[4, 6], x[8] = math.inf, -math.inf, -math.inf
+    rows, plan = zb.sort_tokens(x, ids, 6)
+    at = plan.position.long()
+    assert torch.equal(rows[at], x[:, None, :].expand(T, K, H))
+    w = randn((T, K), g)
+    w[8] = torch.tensor([1.0, 2.0, 0.5, 3.0], device="cuda")
+    r, w = rows.clone().requires_grad_(True), w.requires_grad_(True)
+    y = zb.unsort_tokens(r, plan, w)
+    want = (rows.double()[at] * w.detach().double()[..., None]).sum(1)
+    assert same_places(y.detach().double(), want) and bool((y[8] == -math.inf).all())
+    dy = randn((T, H), g, dtype)
+    dy[2], dy[11, 7] = math.inf, -math.inf
+    dr, dw = torch.autograd.grad(y, (r, w), dy)
+    assert same_places(dr[at].double(), w.detach().double()[..., None] * dy.double()[:, None, :])
+    assert same_places(dw.double(), (rows.double()[at] * dy.double()[:, None, :]).sum(2))
+    grads = [x.clone()]
+    assert math.isinf(float(zb.grad_norm(grads))) and float(zb.grad_norm([-x[:3].float(), torch.full((1,), -math.inf, device="cuda")])) == math.inf
+
+
 # -------------------------------------------------------------------------------------------------- experts' products
 @pytest.mark.parametrize("act, experts, most, H, I", [("swiglu", 200, 150, 512, 256), ("gelu", 97, 400, 1032, 264), ("swiglu", 600, 31, 256, 128)])
 def test_expert_ffn_rows_of_neighbours_never_reach_a_weight_gradient(act, experts, most, H, I):
