@@ -136,6 +136,26 @@ def test_sort_with_an_empty_group_table():
     assert not torch.autograd.grad(rows, x, torch.ones_like(rows))[0].any()
 
 
+# ------------------------------------------------------------------------------------------------------- refusals
+def test_sizes_beyond_the_limits_are_refused():
+    """Before anything is allocated or launched, with the error that the other arguments have."""
+    one = torch.zeros((), dtype=torch.bfloat16, device="cuda")
+    zero = torch.zeros((), dtype=torch.int32, device="cuda")
+    H = (1 << 20) + 8
+    plan = ops.SortPlan(zero.expand(5), zero.expand(1, 2))
+    many = ops.SortPlan(zero.expand(5), zero.expand(1 << 30, 2))
+    for call in (
+            lambda: zb.sort_tokens(one.expand(1, H), zero.expand(1, 2), 4),
+            lambda: zb.sort_tokens(one.expand(1 << 30, 8), zero.expand(1 << 30, 2), 4),
+            lambda: zb.unsort_tokens(one.expand(2, H), plan),
+            lambda: zb.unsort_tokens(one.expand(1 << 31, 8), many),
+            lambda: zb.expert_ffn(one.expand(2, H), zero.expand(2), one.expand(1, 16, H), one.expand(1, H, 8)),
+            lambda: zb.expert_ffn(one.expand(2, 8), zero.expand(2), one.expand(1, H, 8), one.expand(1, 8, H), act="gelu"),
+            lambda: zb.expert_ffn(one.expand(1 << 31, 8), zero.expand(2), one.expand(1, 16, 8), one.expand(1, 8, 8))):
+        with pytest.raises(AssertionError, match="2\\^31|up to|at most"):
+            call()
+
+
 # ------------------------------------------------------------------------------------------------- waits that run out
 @pytest.fixture
 def no_patience():

@@ -35,6 +35,7 @@ _ACTS = {"gelu": 0, "swiglu": 1}
 MAX_GATE_EXPERTS, MAX_GATE_TOPK = 1024, 32
 MAX_SORT_EXPERTS, MAX_SORT_TOPK = 2048, 64
 MAX_FFN_EXPERTS = 1024
+MAX_HIDDEN, MAX_ROWS = 1 << 20, (1 << 31) - 1      # of a row; of the sorted rows
 
 _P, _I, _L, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 _ARGS = {
@@ -239,11 +240,13 @@ def sort_tokens(x, ids, num_experts, group_of=None):
     Copies of an expert keep the order of (token, k).  ids [T, K] int32; a copy whose id is not one of the experts
     (the layer's pads have -1) gets no row, and rows that no copy fills are zero, at the end.  group_of: an int32 table
     that names the group of each id (such as a layer's slot of each expert); `num_experts` then counts groups.
-    Differentiable in x.  K <= 64, at most 2048 experts, T*K < 2^31."""
+    Differentiable in x.  K <= 64, H <= 2^20, at most 2048 experts, T*K < 2^31."""
     if x.dim() != 2 or not x.is_cuda or x.dtype not in _TYPES or x.shape[1] < 1:
         _refuse(f"x: a CUDA tensor [tokens, hidden] of float32, bfloat16 or float16, got {tuple(x.shape)} {x.dtype} {x.device}")
     if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[0] != x.shape[0] or not 1 <= ids.shape[1] <= MAX_SORT_TOPK:
         _refuse(f"ids: int32 [{x.shape[0]}, 1..{MAX_SORT_TOPK}], got {tuple(ids.shape)} {ids.dtype}")
+    if x.shape[1] > MAX_HIDDEN or x.shape[0] * ids.shape[1] > MAX_ROWS:
+        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 copies, got {tuple(x.shape)} and {tuple(ids.shape)}")
     if not 1 <= num_experts <= MAX_SORT_EXPERTS:
         _refuse(f"1..{MAX_SORT_EXPERTS} experts, got {num_experts}")
     if group_of is not None:
@@ -265,6 +268,8 @@ def unsort_tokens(rows, plan, weights=None):
     T, K = plan.position.shape
     if rows.dim() != 2 or not rows.is_cuda or rows.dtype not in _TYPES or rows.shape[0] != T * K or rows.shape[1] < 1:
         _refuse(f"rows: [{T * K}, hidden] of float32, bfloat16 or float16, got {tuple(rows.shape)} {rows.dtype} {rows.device}")
+    if rows.shape[1] > MAX_HIDDEN or T * K > MAX_ROWS:
+        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 of them, got {tuple(rows.shape)}")
     if plan.position.dtype != torch.int32 or plan.offsets.dtype != torch.int32 or not 1 <= K <= MAX_SORT_TOPK:
         _refuse("plan: as sort_tokens returns it")
     if weights is not None:
@@ -326,7 +331,7 @@ def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
     offsets[e] .. offsets[e + 1] go through w1[e] [ffn1, H] and w2[e] [H, ffn] (ffn1 = 2 ffn for "swiglu": gate rows, then
     up rows, as the layer holds them; ffn for "gelu").  All bfloat16, accumulated in float32; offsets int32 [experts + 1]
     on the device, not decreasing, starting at 0; rows behind the last expert's give zero.  hidden and ffn are
-    multiples of 8; at most 1024 experts.  Differentiable in rows, w1 and w2; an expert without rows has a zero gradient."""
+    multiples of 8, up to 2^20 and 2^19; at most 1024 experts, fewer than 2^31 rows.  Differentiable in rows, w1 and w2; an expert without rows has a zero gradient."""
     if act not in _ACTS:
         _refuse(f"act: one of {tuple(_ACTS)}, got {act!r}")
     if not rows.is_cuda or rows.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
@@ -339,6 +344,8 @@ def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
         _refuse("rows and weights are bfloat16, offsets int32")
     if H % 8 or I % 8 or H < 8 or I < 8 or not 1 <= G <= MAX_FFN_EXPERTS:
         _refuse(f"hidden and ffn are multiples of 8, 1..{MAX_FFN_EXPERTS} experts, got {H}, {I}, {G}")
+    if H > MAX_HIDDEN or I > MAX_HIDDEN // 2 or rows.shape[0] > MAX_ROWS:
+        _refuse(f"hidden up to {MAX_HIDDEN}, ffn up to {MAX_HIDDEN // 2}, fewer than 2^31 rows, got {H}, {I}, {rows.shape[0]}")
     _on(rows.device, offsets, w1, w2)
     _no_tangents(rows, w1, w2)
     args = (_dense16(rows), offsets.contiguous(), _dense16(w1), _dense16(w2), _ACTS[act])
