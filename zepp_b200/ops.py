@@ -16,6 +16,7 @@ Where a backward pass is captured into a graph, make the forward pass that it be
 leaves that no graph outside of it still holds (torch runs a leaf's accumulation on the stream of the leaf's first use).
 """
 import ctypes
+import operator
 import threading
 from typing import NamedTuple
 
@@ -54,6 +55,7 @@ _ARGS = {
 }
 # a small call is bound by the host: these two cost a tenth of torch.cuda.current_device() and current_stream()
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_requires_grad = operator.attrgetter("requires_grad")
 _SIZES = ("zepp_op_sort_ws_ints", "zepp_op_grad_norm_ws_bytes")
 _fns = {}
 
@@ -391,17 +393,21 @@ def _norm(tensors, max_norm):
         at = [ctypes.addressof(t) for t in tables]
     else:
         ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), np.uint64, n)
-        sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.int64, n)
+        sizes = np.fromiter(map(torch.Tensor.numel, tensors), np.uint64, n)      # the same bytes as int64
         if len(kinds) == 1:
             types = np.full(n, _TYPES[dtypes[0]], np.uint8)
         else:
             types = np.fromiter(map(_TYPES.__getitem__, dtypes), np.uint8, n)
         if max_norm >= 0:
-            some = sizes > 0
-            first = ptrs[some]
-            last = first + (sizes[some] * np.where(types[some] == 0, 4, 2)).astype(np.uint64)
-            order = first.argsort()
-            overlap = (first[order[1:]] < last[order[:-1]]).any()
+            first, last = ptrs, ptrs + sizes * (np.uint64(4) >> (types != 0))
+            some = sizes != 0
+            if not some.all():
+                first, last = first[some], last[some]
+            if (first[1:] < last[:-1]).any():              # not one behind the other as they are
+                order = first.argsort()
+                overlap = (first[order[1:]] < last[order[:-1]]).any()
+            else:
+                overlap = False
         at = [t.ctypes.data for t in (ptrs, sizes, types)]
     if max_norm >= 0 and overlap:
         _refuse("tensors that do not overlap (one is given twice?)")
@@ -427,7 +433,7 @@ def clip_grad_norm_(tensors, max_norm):
     if not max_norm >= 0.0:
         _refuse(f"max_norm: not negative, got {max_norm}")
     tensors = list(tensors)
-    if any([t.requires_grad and t.is_leaf for t in tensors]):
+    if any(map(_requires_grad, tensors)) and any(t.requires_grad and t.is_leaf for t in tensors):
         _refuse("gradients, not the parameters that they belong to: a tensor is a leaf that requires a gradient")
     out = _norm(tensors, max_norm)
     torch.autograd.graph.increment_version(tensors)      # graphs that saved a tensor learn that it changed
