@@ -98,6 +98,36 @@ def test_infinities_keep_their_sign(dtype):
     assert math.isinf(float(zb.grad_norm(grads))) and float(zb.grad_norm([-x[:3].float(), torch.full((1,), -math.inf, device="cuda")])) == math.inf
 
 
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("T, K, H, dtype", [(650, 11, 2056, torch.float16), (592, 1, 2048, torch.bfloat16), (593, 9, 6152, torch.bfloat16), (1200, 24, 2048, torch.float16),
+                                            (591, 8, 4096, torch.bfloat16), (700, 8, 1024, torch.bfloat16), (700, 3, 4096, torch.float32)])
+def test_unsort_gradient_of_long_rows(T, K, H, dtype):
+    """Both ways that the gradient of long rows is computed: whole pieces and ragged ones, one copy and more than eight, tokens
+    without any, the two results together and each alone."""
+    g = gen(T + K)
+    ids = torch.randint(-1, 40, (T, K), generator=g, device="cuda", dtype=torch.int32)
+    ids[7], ids[T - 1] = -1, -1
+    _, plan = zb.sort_tokens(randn((T, 8), g), ids, 40)
+    r, w, dy = randn((T * K, H), g, dtype).requires_grad_(True), randn((T, K), g).requires_grad_(True), randn((T, H), g, dtype)
+    dr, dw = torch.autograd.grad(zb.unsort_tokens(r, plan, w), (r, w), dy)
+    half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny
+    dr64 = torch.zeros((T * K, H), dtype=torch.float64, device="cuda")
+    for k in range(K):
+        p = plan.position[:, k].long()
+        t = (p >= 0).nonzero()[:, 0]
+        dr64[p[t]] = w.detach()[t, k, None].double() * dy[t].double()
+        d = r.detach()[p.clamp_min(0)].double() * dy.double() * (p >= 0)[:, None]
+        # a thread adds at most H / 32 products one after the other, then 5 + 8 sums join them
+        bound = (H / 32 + 8 + 13) * U * d.abs().sum(1) + 1e-30
+        assert bool(((dw[:, k].double() - d.sum(1)).abs() <= bound).all()) and bool((dw[p < 0, k] == 0).all())
+    assert bool(((dr.double() - dr64).abs() <= (half + 2 * U) * dr64.abs() + tiny).all())
+    assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r, plan, w.detach()), r, dy)[0], dr)
+    assert torch.equal(torch.autograd.grad(zb.unsort_tokens(r.detach(), plan, w), w, dy)[0], dw)
+    ops.check_waits()
+
+
 # -------------------------------------------------------------------------------------------------- experts' products
 @pytest.mark.parametrize("act, experts, most, H, I", [("swiglu", 200, 150, 512, 256), ("gelu", 97, 400, 1032, 264), ("swiglu", 600, 31, 256, 128)])
 def test_expert_ffn_rows_of_neighbours_never_reach_a_weight_gradient(act, experts, most, H, I):

@@ -322,23 +322,21 @@ __global__ void __launch_bounds__(kUnsortGradThreads) unsort_grad_kernel(const U
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The same two for long rows in large numbers: one persistent block per SM, a warp that fetches pieces of the rows into a
-// ring of shared-memory stages with bulk copies, eight warps that add them up.  A stage holds one piece (kPieceBytes) of up
-// to eight copies' rows (GRAD: and of dy), so nearly 200 KB are in flight on every SM whatever the registers allow: 112 and
-// 185 us where the kernels above take 152 and 226 (8192 tokens x 8 copies of 4096 bf16).
-// Steps of a block, `steps` in all per token: (piece, eight copies) with the copies inner, or GRAD: (eight copies, piece)
-// with the piece inner, so that a sum over k or over the row stays in registers.
+// The gradient once more, for long rows of 16-bit elements in large numbers: one persistent block per SM, a warp that fetches
+// pieces of the rows into a ring of shared-memory stages with bulk copies, eight warps that work on them.  A stage holds one
+// piece (kPieceBytes) of dy and of up to eight copies' rows, so nearly 200 KB are in flight on every SM whatever the
+// registers allow, where the kernel above waits for its loads: 190 us against 235 (8192 tokens x 8 copies of 4096 bf16).
+// Steps of a token: (eight copies, piece) with the piece inner, so that a sum over the row stays in registers.
 constexpr int kPieceBytes = 4096;
 constexpr int kPieceThreads = kPieceBytes / 16;         // consumers: a 16-byte vector each
 constexpr int kBulkThreads = 32 + kPieceThreads;
-constexpr int kBulkMaxStages = 16;
-constexpr int kBulkRingBytes = 48 * kPieceBytes;        // six stages, five with dy
+constexpr int kBulkStageBytes = 9 * kPieceBytes;        // eight copies and dy
+constexpr int kBulkStages = 5;
 constexpr unsigned long long kBulkDrainNs = 2000000000ull;      // limit of each wait for copies after a role gave up
 
 struct BulkArgs {
   UnsortArgs u;
   int pieces, chunks;         // of a row; of its copies, eight at a time
-  int stages, stage_bytes;
   unsigned long long* status;
   unsigned long long limit_ns;
 };
@@ -348,33 +346,32 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const BulkArgs b) {
+template <typename T>
+__global__ void __launch_bounds__(kBulkThreads, 1) unsort_grad_bulk_kernel(const BulkArgs b) {
   constexpr int E = 16 / (int)sizeof(T);
   typedef Pack<T, E> V;
   const UnsortArgs& a = b.u;
   extern __shared__ __align__(128) unsigned char bulk_ring[];
-  __shared__ __align__(8) uint64_t full[kBulkMaxStages], empty[kBulkMaxStages];
-  __shared__ int s_pos[kBulkMaxStages][8];
-  __shared__ float s_w[kBulkMaxStages][8];
+  __shared__ __align__(8) uint64_t full[kBulkStages], empty[kBulkStages];
+  __shared__ int s_pos[kBulkStages][8];
+  __shared__ float s_w[kBulkStages][8];
   __shared__ float s_dot[2][kPieceThreads / 32][8];
   __shared__ int abort_flag;
   volatile int* abortp = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < b.stages; ++i) {
+    for (int i = 0; i < kBulkStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kPieceThreads / 32);
     }
     fence_barrier_init();
   }
   __syncthreads();
-  // without GRAD a token's pieces are independent: blocks share them out
-  const int per_unit = GRAD ? b.pieces * b.chunks : b.chunks;
-  const int units = (int)(GRAD ? a.T : a.T * b.pieces);        // rows of 2 KB and more: far fewer than 2^31 fit the memory
-  const int mine = (units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;      // gridDim.x <= units
-  const int total = mine * per_unit;
+  const int per_token = b.pieces * b.chunks;
+  // gridDim.x <= T; rows of 4 KB and more: far fewer than 2^31 fit the memory
+  const int mine = ((int)a.T - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int total = mine * per_token;
   const long long row_bytes = a.H * (long long)sizeof(T);
   int issued = 0;                                              // warp 0: stages whose copies it has started
 
@@ -382,7 +379,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
     // ---------------------------------------------------------------- copies
     // Positions and weights of four steps at a time (lane: step lane / 8, copy lane % 8), four steps ahead: they are the
     // first link of every chain of loads, and one step ahead each stage still waited for most of their latency.
-    int unit = blockIdx.x, step = 0, stage = 0;
+    int token = blockIdx.x, step = 0, stage = 0;
     uint32_t phase = 0;
     int p_next = -1, p_four = -1;
     float w_next = 1.0f, w_four = 1.0f;
@@ -391,9 +388,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
       p_next = -1;
       w_next = 1.0f;
       if (i < total) {
-        const int u = (int)blockIdx.x + i / per_unit * (int)gridDim.x, st = i % per_unit;
-        const int k = (GRAD ? st / b.pieces : st) * 8 + (lane & 7);
-        const long long at = (long long)(GRAD ? u : u / b.pieces) * a.K + k;
+        const int k = i % per_token / b.pieces * 8 + (lane & 7);
+        const long long at = (long long)((int)blockIdx.x + i / per_token * (int)gridDim.x) * a.K + k;
         if (k < a.K) {
           p_next = unsort_position(a, at);
           if (a.weights != nullptr) w_next = a.weights[at];
@@ -411,11 +407,10 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
       const int p_lane = __shfl_sync(0xffffffffu, p_four, from);
       const int now_p = lane < 8 ? p_lane : -1;
       const float now_w = __shfl_sync(0xffffffffu, w_four, from);
-      const int piece = GRAD ? step % b.pieces : unit % b.pieces;
-      const long long t = GRAD ? unit : unit / b.pieces;
-      const uint32_t at = (uint32_t)piece * kPieceBytes;
+      const long long t = token;
+      const uint32_t at = (uint32_t)(step % b.pieces) * kPieceBytes;
       const uint32_t bytes = (uint32_t)min((long long)kPieceBytes, row_bytes - at);
-      if (++step == per_unit) { step = 0; unit += gridDim.x; }
+      if (++step == per_token) { step = 0; token += gridDim.x; }
       const bool ok = mbar_wait_bounded(&empty[stage], phase ^ 1, abortp, b.limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) {
@@ -428,115 +423,90 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
         s_pos[stage][lane] = now_p;
         s_w[stage][lane] = now_w;
       }
-      const bool rows = !GRAD || a.dweights != nullptr;
+      const bool rows = a.dweights != nullptr;
       const uint32_t copies = rows ? __popc(__ballot_sync(0xffffffffu, now_p >= 0)) : 0u;
       __syncwarp();
-      if (lane == 0) mbar_expect_tx(&full[stage], (copies + (GRAD ? 1u : 0u)) * bytes);
+      if (lane == 0) mbar_expect_tx(&full[stage], (copies + 1u) * bytes);
       __syncwarp();
-      unsigned char* st = bulk_ring + (size_t)stage * b.stage_bytes;
+      unsigned char* st = bulk_ring + (size_t)stage * kBulkStageBytes;
       if (rows && now_p >= 0)
         bulk_load(st + lane * kPieceBytes, static_cast<const unsigned char*>(a.rows) + now_p * row_bytes + at, bytes, &full[stage]);
-      if (GRAD && lane == 8)
+      if (lane == 8)
         bulk_load(st + 8 * kPieceBytes, static_cast<const unsigned char*>(a.dy) + t * row_bytes + at, bytes, &full[stage]);
       ++issued;
-      if (++stage == b.stages) { stage = 0; phase ^= 1; }
+      if (++stage == kBulkStages) { stage = 0; phase ^= 1; }
     }
   } else {
     // ---------------------------------------------------------------- sums
     const int v = threadIdx.x - 32;
-    int unit = blockIdx.x, step = 0, stage = 0, flip = 0;
+    int token = blockIdx.x, step = 0, stage = 0, flip = 0;
     uint32_t phase = 0;
-    float acc[GRAD ? 8 : E];
+    float acc[8];
 #pragma unroll
-    for (int e = 0; e < (GRAD ? 8 : E); ++e) acc[e] = 0.0f;
+    for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
     for (int i = 0; i < total; ++i) {
-      const int piece = GRAD ? step % b.pieces : unit % b.pieces;
-      const int chunk = GRAD ? step / b.pieces : step;
-      const long long t = GRAD ? unit : unit / b.pieces;
+      const int piece = step % b.pieces, chunk = step / b.pieces;
+      const long long t = token;
       const long long at = (long long)piece * kPieceBytes + v * 16;
       const bool in = at < row_bytes;
       const bool ok = mbar_wait_bounded(&full[stage], phase, abortp, b.limit_ns);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0 && !*abortp) record_timeout(b.status, WAIT_MBAR_FULL, t, i);
         abort_flag = 1;
-        if (GRAD) asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");      // nobody is left waiting below
+        asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");      // nobody is left waiting below
         break;
       }
-      const unsigned char* st = bulk_ring + (size_t)stage * b.stage_bytes + v * 16;
-      if (GRAD) {
-        if (in) {
-          const V d = *reinterpret_cast<const V*>(st + 8 * kPieceBytes);
-          float f[E];
+      const unsigned char* st = bulk_ring + (size_t)stage * kBulkStageBytes + v * 16;
+      if (in) {
+        const V d = *reinterpret_cast<const V*>(st + 8 * kPieceBytes);
+        float f[E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = to_f32<T>(d.v[e]);
+        for (int e = 0; e < E; ++e) f[e] = to_f32<T>(d.v[e]);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int p = s_pos[stage][q];
-            if (p >= 0) {
-              if (a.dweights != nullptr) {
-                const V r = *reinterpret_cast<const V*>(st + q * kPieceBytes);
+        for (int q = 0; q < 8; ++q) {
+          const int p = s_pos[stage][q];
+          if (p >= 0) {
+            if (a.dweights != nullptr) {
+              const V r = *reinterpret_cast<const V*>(st + q * kPieceBytes);
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[q] = fmaf(f[e], to_f32<T>(r.v[e]), acc[q]);
-              }
-              if (a.drows != nullptr) {
-                const float w = s_w[stage][q];
-                V o;
+              for (int e = 0; e < E; ++e) acc[q] = fmaf(f[e], to_f32<T>(r.v[e]), acc[q]);
+            }
+            if (a.drows != nullptr) {
+              const float w = s_w[stage][q];
+              V o;
 #pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(w * f[e]);
-                *reinterpret_cast<V*>(static_cast<unsigned char*>(a.drows) + p * row_bytes + at) = o;
-              }
+              for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(w * f[e]);
+              *reinterpret_cast<V*>(static_cast<unsigned char*>(a.drows) + p * row_bytes + at) = o;
             }
           }
         }
-      } else if (in) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (s_pos[stage][q] >= 0) {
-            const V r = *reinterpret_cast<const V*>(st + q * kPieceBytes);
-            const float w = s_w[stage][q];
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, to_f32<T>(r.v[e]), acc[e]);
-          }
       }
-      const int p_of_lane = GRAD && lane < 8 ? s_pos[stage][lane] : -1;
+      const int p_of_lane = lane < 8 ? s_pos[stage][lane] : -1;
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
-      if (++stage == b.stages) { stage = 0; phase ^= 1; }
-      if (GRAD) {
-        if (piece == b.pieces - 1) {                           // eight copies of a token are done
-          if (a.dweights != nullptr) {
+      if (++stage == kBulkStages) { stage = 0; phase ^= 1; }
+      if (piece == b.pieces - 1 && a.dweights != nullptr) {    // eight copies of a token are done
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float s = warp_sum(acc[q]);
-              if (lane == q) s_dot[flip][warp - 1][q] = s;
-              acc[q] = 0.0f;
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kPieceThreads) : "memory");
-            if (__any_sync(0xffffffffu, *abortp)) {            // a warp that gave up has left: go too, and count for the next round
-              asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");
-              break;
-            }
-            if (warp == 1 && lane < 8 && chunk * 8 + lane < a.K) {
-              float s = 0.0f;
-              for (int w = 0; w < kPieceThreads / 32; ++w) s += s_dot[flip][w][lane];
-              a.dweights[t * a.K + chunk * 8 + lane] = p_of_lane >= 0 ? s : 0.0f;
-            }
-            flip ^= 1;                                         // the other half is free: its readers passed this barrier
-          }
+        for (int q = 0; q < 8; ++q) {
+          const float s = warp_sum(acc[q]);
+          if (lane == q) s_dot[flip][warp - 1][q] = s;
+          acc[q] = 0.0f;
         }
-      } else if (chunk == b.chunks - 1) {
-        if (in) {
-          V o;
-#pragma unroll
-          for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(acc[e]);
-          *reinterpret_cast<V*>(static_cast<unsigned char*>(a.y) + t * row_bytes + at) = o;
+        asm volatile("bar.sync 1, %0;" ::"n"(kPieceThreads) : "memory");
+        if (__any_sync(0xffffffffu, *abortp)) {                // a warp that gave up has left: go too, and count for the next round
+          asm volatile("bar.arrive 1, %0;" ::"n"(kPieceThreads) : "memory");
+          break;
         }
-#pragma unroll
-        for (int e = 0; e < (GRAD ? 8 : E); ++e) acc[e] = 0.0f;
+        if (warp == 1 && lane < 8 && chunk * 8 + lane < a.K) {
+          float s = 0.0f;
+          for (int w = 0; w < kPieceThreads / 32; ++w) s += s_dot[flip][w][lane];
+          a.dweights[t * a.K + chunk * 8 + lane] = p_of_lane >= 0 ? s : 0.0f;
+        }
+        flip ^= 1;                                             // the other half is free: its readers passed this barrier
       }
-      if (++step == per_unit) { step = 0; unit += gridDim.x; }
+      if (++step == per_token) { step = 0; token += gridDim.x; }
     }
-    if (GRAD && a.drows != nullptr) {
+    if (a.drows != nullptr) {
       long long begin = *a.n_rows;
       if (begin < 0) begin = 0;
       for (long long p = begin + blockIdx.x; p < a.N; p += gridDim.x)
@@ -547,8 +517,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1) unsort_bulk_kernel(const Bulk
   __syncthreads();
   if (warp == 0 && *abortp) {                                  // a role gave up: the block stays until its copies have landed
     int never = 0;
-    for (int i = issued > b.stages ? issued - b.stages : 0; i < issued; ++i)
-      mbar_wait_bounded(&full[i % b.stages], (uint32_t)(i / b.stages) & 1u, &never, kBulkDrainNs);
+    for (int i = issued > kBulkStages ? issued - kBulkStages : 0; i < issued; ++i)
+      mbar_wait_bounded(&full[i % kBulkStages], (uint32_t)(i / kBulkStages) & 1u, &never, kBulkDrainNs);
   }
 }
 

@@ -51,9 +51,7 @@ cudaError_t ffn_smem() {
 
 template <typename T>
 cudaError_t bulk_smem() {
-  cudaError_t e = cudaFuncSetAttribute(unsort_bulk_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkRingBytes);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(unsort_bulk_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkRingBytes);
+  return cudaFuncSetAttribute(unsort_grad_bulk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkStages * kBulkStageBytes);
 }
 
 // the current device's record; its first use sets kernel attributes and looks up the status block
@@ -81,7 +79,6 @@ int op_device(OpDevice** out) {
     CU_OK(ffn_smem<FFN_DACT_GELU>());
     CU_OK(ffn_smem<FFN_DROWS>());
     CU_OK(ffn_smem<FFN_DWEIGHT>());
-    CU_OK(bulk_smem<float>());
     CU_OK(bulk_smem<__nv_bfloat16>());
     CU_OK(bulk_smem<__half>());
     d.ready = true;
@@ -256,28 +253,31 @@ static void unsort_launch(const UnsortArgs& a, bool grad, int sms, cudaStream_t 
     unsort_kernel<T, E, E == 1 ? 4 : 1, 8><<<grid, kUnsortThreads, 0, s>>>(a);
   }
 }
-// pieces of rows through shared memory: worth it for rows of half a piece or more, once every block has several
-template <typename T, bool GRAD>
-static bool unsort_bulk(const UnsortArgs& a, const OpDevice* d, cudaStream_t s) {
+// The gradient through the ring of shared-memory stages, where that is faster.  Measured against the kernel above, which it
+// replaces then (us, 128 experts, T tokens x 8 copies, rows from HBM):
+//   bf16, rows of 2 KB:  T 592 10.4 / 10.2, T 9472 100 / 80        of 4 KB:  T 592 12.5 / 15.9, T 9472 110 / 150
+//         rows of 8 KB:  T 148 8.5 / 12.3 (one copy, T 300: 8.0 / 7.2), T 592 19.8 / 26.3, T 9472 243 / 282
+//   fp32, rows of 4 KB:  T 592 11.5 / 9.7, T 9472 128 / 109        of 8 KB:  T 592 18.8 / 16.6, T 9472 239 / 214
+// (half as many elements in the same bytes: nothing is left to win).  Without the weights' gradient the two are within 15 %.
+template <typename T>
+static bool unsort_grad_bulk(const UnsortArgs& a, const OpDevice* d, cudaStream_t s) {
   const long long row_bytes = a.H * (long long)sizeof(T);
+  if (row_bytes < kPieceBytes || a.T < 4ll * d->sms) return false;
   BulkArgs b{};
   b.u = a;
   b.pieces = (int)((row_bytes + kPieceBytes - 1) / kPieceBytes);
   b.chunks = (a.K + 7) / 8;
-  const long long units = GRAD ? a.T : a.T * b.pieces;
-  if (row_bytes * 2 < kPieceBytes || units < 4ll * d->sms) return false;
-  b.stage_bytes = (GRAD ? 9 : 8) * kPieceBytes;
-  b.stages = kBulkRingBytes / b.stage_bytes;
   b.status = d->status;
   b.limit_ns = g_op_wait_ns;
-  unsort_bulk_kernel<T, GRAD><<<d->sms, kBulkThreads, b.stages * b.stage_bytes, s>>>(b);
+  unsort_grad_bulk_kernel<T><<<d->sms, kBulkThreads, kBulkStages * kBulkStageBytes, s>>>(b);
   return true;
 }
 template <typename T>
 static void unsort_type(const UnsortArgs& a, bool grad, const OpDevice* d, cudaStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   const bool wide = a.H % E == 0 && aligned(a.rows, 16) && aligned(a.y, 16) && aligned(a.dy, 16) && aligned(a.drows, 16);
-  if (wide && (grad ? unsort_bulk<T, true>(a, d, s) : unsort_bulk<T, false>(a, d, s))) return;
+  if constexpr (sizeof(T) == 2)
+    if (wide && grad && unsort_grad_bulk<T>(a, d, s)) return;
   if (wide) unsort_launch<T, E>(a, grad, d->sms, s);
   else unsort_launch<T, 1>(a, grad, d->sms, s);
 }
