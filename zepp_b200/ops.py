@@ -243,12 +243,13 @@ def sort_tokens(x, ids, num_experts, group_of=None):
     (the layer's pads have -1) gets no row, and rows that no copy fills are zero, at the end.  group_of: an int32 table
     that names the group of each id (such as a layer's slot of each expert); `num_experts` then counts groups.
     Differentiable in x.  K <= 64, H <= 2^20, at most 2048 experts, T*K < 2^31."""
-    if x.dim() != 2 or not x.is_cuda or x.dtype not in _TYPES or x.shape[1] < 1:
+    xs, s = x.shape, ids.shape
+    if len(xs) != 2 or not x.is_cuda or x.dtype not in _TYPES or xs[1] < 1:
         _refuse(f"x: a CUDA tensor [tokens, hidden] of float32, bfloat16 or float16, got {tuple(x.shape)} {x.dtype} {x.device}")
-    if ids.dim() != 2 or ids.dtype != torch.int32 or ids.shape[0] != x.shape[0] or not 1 <= ids.shape[1] <= MAX_SORT_TOPK:
-        _refuse(f"ids: int32 [{x.shape[0]}, 1..{MAX_SORT_TOPK}], got {tuple(ids.shape)} {ids.dtype}")
-    if x.shape[1] > MAX_HIDDEN or x.shape[0] * ids.shape[1] > MAX_ROWS:
-        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 copies, got {tuple(x.shape)} and {tuple(ids.shape)}")
+    if len(s) != 2 or ids.dtype != torch.int32 or s[0] != xs[0] or not 1 <= s[1] <= MAX_SORT_TOPK:
+        _refuse(f"ids: int32 [{xs[0]}, 1..{MAX_SORT_TOPK}], got {tuple(s)} {ids.dtype}")
+    if xs[1] > MAX_HIDDEN or s[0] * s[1] > MAX_ROWS:
+        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 copies, got {tuple(xs)} and {tuple(s)}")
     if not 1 <= num_experts <= MAX_SORT_EXPERTS:
         _refuse(f"1..{MAX_SORT_EXPERTS} experts, got {num_experts}")
     if group_of is not None:
@@ -268,10 +269,11 @@ def unsort_tokens(rows, plan, weights=None):
     that have a row, added up in float32 in the order of k.  weights [T, K] float32; without them every copy counts once.
     Differentiable in rows and weights."""
     T, K = plan.position.shape
-    if rows.dim() != 2 or not rows.is_cuda or rows.dtype not in _TYPES or rows.shape[0] != T * K or rows.shape[1] < 1:
-        _refuse(f"rows: [{T * K}, hidden] of float32, bfloat16 or float16, got {tuple(rows.shape)} {rows.dtype} {rows.device}")
-    if rows.shape[1] > MAX_HIDDEN or T * K > MAX_ROWS:
-        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 of them, got {tuple(rows.shape)}")
+    s = rows.shape
+    if len(s) != 2 or not rows.is_cuda or rows.dtype not in _TYPES or s[0] != T * K or s[1] < 1:
+        _refuse(f"rows: [{T * K}, hidden] of float32, bfloat16 or float16, got {tuple(s)} {rows.dtype} {rows.device}")
+    if s[1] > MAX_HIDDEN or s[0] > MAX_ROWS:
+        _refuse(f"rows of at most {MAX_HIDDEN} elements, fewer than 2^31 of them, got {tuple(s)}")
     if plan.position.dtype != torch.int32 or plan.offsets.dtype != torch.int32 or not 1 <= K <= MAX_SORT_TOPK:
         _refuse("plan: as sort_tokens returns it")
     if weights is not None:
@@ -378,7 +380,8 @@ def _norm(tensors, max_norm):
         _refuse("CUDA tensors of one device, of float32, bfloat16 or float16")
     if not all(map(torch.Tensor.is_contiguous, tensors)) and not all(t.is_contiguous() or _is_dense(t) for t in tensors):
         _refuse("tensors whose elements lie without gaps and only once in memory")
-    _no_tangents(*tensors)
+    if forward_ad._current_level >= 0:
+        _no_tangents(*tensors)
     n = len(tensors)
     out = torch.empty((), dtype=torch.float32, device=device)
     ws = torch.empty(_fn("zepp_op_grad_norm_ws_bytes")(n), dtype=torch.uint8, device=device)
@@ -415,14 +418,12 @@ def _norm(tensors, max_norm):
     return out
 
 
-@torch.no_grad()
 def grad_norm(tensors):
     """The 2-norm over all elements of the tensors (float32, bfloat16 and float16 may be mixed), a float32 scalar on their
-    device; sums run in 64 bits across chunks and in a fixed order."""
+    device; sums run in 64 bits across chunks and in a fixed order.  Not differentiable."""
     return _norm(tensors, -1.0)
 
 
-@torch.no_grad()
 def clip_grad_norm_(tensors, max_norm):
     """Scale the tensors in place by min(1, max_norm / (norm + 1e-6)), norm being grad_norm(tensors), which is returned.
     The tensors are the gradients themselves, not parameters: leaves that require a gradient are refused.
