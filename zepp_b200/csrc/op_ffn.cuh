@@ -23,7 +23,7 @@
 // and leave as contiguous pieces of a row.  Every wait is bounded.
 //
 // Measured (B200, 32768 rows of 128 experts, H 2048, I 768, SwiGLU): h and a 222 us, y 116, dh 150, dx 200, dW2 128, dW1 229;
-// HBM alone, with reads at 6.5 TB/s and writes at about 4.2, would take 204, 102, 144, 171, 124, 228.  With thousands of rows
+// HBM alone, with reads at 6.5 TB/s and writes at about 4.2, would take 204, 102, 138, 171, 124, 228.  With thousands of rows
 // per expert: 1.2 to 1.5 PFLOP/s (cuBLAS on one large product: 1.65).
 //
 // Roundings: products accumulate in fp32; h is kept as it is, in fp32, for the backward pass (in bf16 its rounding made the

@@ -11,8 +11,13 @@
 // A warp owns a row and holds it in registers, so the logits are read once: element (j / 4) * 128 + lane * 4 + j % 4 for
 // register j, four neighbours per access.  The (k + 1)-th largest of the 32 lanes' largest keys (order-preserving
 // integers, redux.sync) is a bound that hardly more than k keys reach; those few are put together, one per lane, and each
-// counts the ones before it (up to k = 20 or so they are fewer than 32; a row with more goes through 64 bits).  That is about 20 instructions per place, where k rounds of a maximum over all registers took
-// 200 (16381 rows of 384 bf16 logits with a bias: 25 us against 45 us).  Bound by instruction issue.
+// counts the ones before it.  That is about 20 instructions per place, where k rounds of a maximum over all registers took
+// 200 (16381 rows of 384 bf16 logits with a bias: 25 us against 45 us).  A row with more than 32 keys at the bound goes
+// through 64 bits: of normal logits none up to k = 14, 0.4 % with 16, 8 % with 18, 41 % with 20, 83 % with 22 and all with 28;
+// and rows of equal logits.  The same 16381 rows take 23 us with k = 8, 24 with 12, 34 with 16, 75 with 20, 104 with 22
+// and 140 with 32; with equal logits and k = 8, 44.
+// 990 instructions a row; the schedulers issue in 65 % of their cycles, and a warp waits longest for results of fixed latency
+// (31 % of its time), for the logits (14 %) and for shared memory, shuffles and reductions (12 %).
 #pragma once
 #include "op_common.cuh"
 
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a)
     if (a.renormalize) {
       sum = warp_sum(w);
     } else {
-      sum = 0.0f;
+      sum = 0.0f;                  // __expf is off by units of 2 + 1.16 |x|: the more, the less the summand counts
 #pragma unroll
       for (int j = 0; j < NPL; ++j) sum += __expf(l[j] - mx);
       sum = warp_sum(sum);
@@ -245,8 +250,8 @@ __global__ void __launch_bounds__(32 * kGateWarps) gate_kernel(const GateArgs a)
 //   softmax, all experts:   dl_g = p_g * (q_g [g chosen] - sum_c q_c p_c)
 //   renormalised, t = sum_c v_c, v = p or s:  dv_c = (q_c - sum_e q_e v_e / t) / t;  dl_c = dv_c v_c (softmax), dv_c s_c (1 - s_c)
 //   sigmoid, not renormalised:  dl_c = q_c s_c (1 - s_c)
-// Only the first has a value for every expert; the others write zeros there and read the chosen logits alone.  Bound by
-// launch and instruction issue (16381 x 384 bf16, sigmoid: 8.8 us; 8192 x 128 fp32, softmax over all: 6.3 us).
+// Only the first has a value for every expert; the others write zeros there and read the chosen logits alone.  Measured:
+// 16381 x 384 bf16, sigmoid, 8.8 us (the bytes take 2.1); 8192 x 128 fp32, softmax over all, 6.3 us (1.3).
 template <typename T, int NPL>
 __global__ void __launch_bounds__(32 * kGateWarps) gate_grad_kernel(const GateArgs a) {
   extern __shared__ __align__(16) unsigned char gate_rows[];       // kGateWarps rows of G elements, 16-byte multiples

@@ -8,9 +8,8 @@
 // The order is that of a stable sort by group, and every sum runs over k in order, so equal inputs give equal bits.
 // Everything is bound by the bytes of the rows: the sort reads a row once and writes its K copies, the gradient of the
 // unsort reads dy once and makes both of its results from one pass over the rows.  Measured with 8192 tokens x 8 copies of
-// 4096 bf16: sort 4 + 119 us (5.1 TB/s, nearly all writes; a fill of memory reaches 3.9), unsort 112 us (5.4 TB/s), its
-// gradient 185 us (6.2 TB/s).  Counting costs the second launch only above 8192 copies; with fewer, a block that counts all
-// ids itself takes less than a launch (32 tokens: 6 us).
+// 4096 bf16: sort 4 + 120 us (5.0 TB/s, nearly all writes; a fill of memory reaches 3.9), unsort 102 us (5.9 TB/s), its
+// gradient 185 us (6.2 TB/s).
 #pragma once
 #include "op_common.cuh"
 
@@ -18,7 +17,10 @@ namespace zepp {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortMaxGroups = 2048;
-constexpr int kSortDirect = 8192;       // up to this many copies every block counts all of them itself: one launch
+// Up to this many copies every block counts all of them itself: one launch.  Against a launch that counts beforehand (128
+// experts, rows of 2048 bf16): 4.1 us against 8.2 for 256 copies, 13.4 against 15.9 for 8192, 22 either way for 16384, 43
+// against 38 for 32768.
+constexpr int kSortDirect = 8192;
 constexpr int kSortChunks = 64;         // above: parts of the copies that are counted beforehand
 
 struct SortArgs {
