@@ -210,7 +210,7 @@ int zepp_op_grad_norm(void* const* ptrs, const int64_t* sizes, const uint8_t* dt
                       float* norm_dev, void* ws_dev, void* stream);
 
 /* How long a bounded wait inside an operator's kernel lasts before the kernel gives up (its outputs are then incomplete and
- * zepp_op_status says so); for the calls of this process from now on, 2 s where nothing was set. */
+ * zepp_op_status says so); for the calls of this process from now on, 2 s where nothing was set, at most an hour. */
 int zepp_op_set_wait_limit_ns(int64_t ns);
 
 /* Deferred verdict of the operators' bounded waits on the current device: synchronises the device, copies 8 status words

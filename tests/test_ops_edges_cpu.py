@@ -16,7 +16,11 @@ def error(rc):
 
 
 def test_wait_limit():
-    assert "wait limit" in error(ops._fn("zepp_op_set_wait_limit_ns")(-1))
+    for ns in (-1, 3600 * 10 ** 9 + 1, 2 ** 62):
+        assert "wait limit" in error(ops._fn("zepp_op_set_wait_limit_ns")(ns))
+    for look in (zb.check_waits, ops.wait_failures):
+        with pytest.raises(AssertionError, match="CUDA device"):
+            look("cpu")
     for bad in (-1.0, float("nan"), float("inf"), 3601):
         with pytest.raises(AssertionError):
             ops.set_wait_limit(bad)

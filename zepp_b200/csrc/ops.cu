@@ -99,7 +99,7 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 }  // namespace
 
 extern "C" int zepp_op_set_wait_limit_ns(int64_t ns) {
-  if (ns < 0) return fail("wait limit: %lld ns", (long long)ns);
+  if (ns < 0 || ns > 3600000000000ll) return fail("wait limit: 0..3600 s (got %lld ns)", (long long)ns);
   g_op_wait_ns = (unsigned long long)ns;
   return 0;
 }

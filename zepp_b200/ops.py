@@ -335,7 +335,8 @@ def expert_ffn(rows, offsets, w1, w2, act="swiglu"):
     offsets[e] .. offsets[e + 1] go through w1[e] [ffn1, H] and w2[e] [H, ffn] (ffn1 = 2 ffn for "swiglu": gate rows, then
     up rows, as the layer holds them; ffn for "gelu").  All bfloat16, accumulated in float32; offsets int32 [experts + 1]
     on the device, not decreasing, starting at 0; rows behind the last expert's give zero.  hidden and ffn are
-    multiples of 8, up to 2^20 and 2^19; at most 1024 experts, fewer than 2^31 rows.  Differentiable in rows, w1 and w2; an expert without rows has a zero gradient."""
+    multiples of 8, up to 2^20 and 2^19; at most 1024 experts, fewer than 2^31 rows.  Differentiable in rows, w1 and w2; an
+    expert without rows has a zero gradient."""
     if act not in _ACTS:
         _refuse(f"act: one of {tuple(_ACTS)}, got {act!r}")
     if not rows.is_cuda or rows.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
@@ -463,6 +464,8 @@ def _status(index):
 
 def _device_index(device):
     device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        _refuse(f"a CUDA device, got {device}")
     return _current_device() if device.index is None else device.index
 
 
